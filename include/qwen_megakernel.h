@@ -241,6 +241,65 @@ int qwen_lm_head_sample(const void* hidden_f16, const void* weight, float temper
 int qwen_mlp_block(const void* x_f16, const void* post_norm_weight, const void* gate_weight,
                    const void* up_weight, const void* down_weight, float* y_out, hipStream_t stream);
 
+/* ---- the head over many positions (no counterpart in the reference) ------------------
+ *
+ * Operators for scoring a text, for training on what the engine computes, and for products in
+ * 8-bit integers. They need no other call's workspace, follow the stream they are given and
+ * nothing else, may run beside every other call, be captured into graphs, and be called from several
+ * threads at once (each with a workspace of its own). They use the current device. */
+
+#define QWEN_F16 0
+#define QWEN_BF16 1
+#define QWEN_F32 2
+
+/* Softmax cross entropy of hidden rows against a head, without keeping the logits: for each of
+ * `tokens` rows h_t of `hidden` ([tokens][hidden_stride], dtype QWEN_F16 or QWEN_BF16) and the rows
+ * w_v of `weight` ([vocab][weight_stride], the same dtype)
+ *   lse[t]  = log sum_v exp(h_t . w_v)                (fp32 [tokens])
+ *   loss[t] = lse[t] - h_t . w_target                 (fp32 [tokens])
+ * and, with `total` (nullable, fp32 [2]), the sum of the losses and the number of positions that
+ * count. targets: device integers of target_bits (32 or 64) bits; a target equal to ignore_index does
+ * not count (loss 0), one outside [0, vocab) otherwise gives a NaN loss. Sums are fp32, in an order
+ * that depends on the sizes only: the same call always gives the same bits.
+ * width: a multiple of 8; the strides (in elements): multiples of 8, at least width and at most
+ * 2097152; hidden, weight and workspace: 16-byte aligned; tokens 0 .. 1048576 (0: nothing is done);
+ * vocab 1 .. 16777216. workspace: device memory of qwen_cross_entropy_workspace() bytes, free for
+ * other use when the call's work has ended. */
+long long qwen_cross_entropy_workspace(int tokens, int vocab, int width);
+int qwen_cross_entropy(const void* hidden, long long hidden_stride, const void* weight, long long weight_stride,
+                       const void* targets, int target_bits, int tokens, int vocab, int width, int dtype,
+                       long long ignore_index, float* loss, float* lse, float* total, void* workspace,
+                       long long workspace_bytes, hipStream_t stream);
+
+/* Its gradients: with p_tv = exp(h_t . w_v - lse[t]) and g_t = grad_loss[t * grad_stride] (fp32; stride
+ * 0: one number for all positions)
+ *   grad_hidden[t] = g_t sum_v (p_tv - [v = target_t]) w_v     ([tokens][width])
+ *   grad_weight[v] = sum_t g_t (p_tv - [v = target_t]) h_t     ([vocab][width])
+ * in the inputs' dtype; either may be null. lse is what qwen_cross_entropy gave for the same inputs.
+ * Positions that do not count take no part (their hidden rows may hold anything) and get a zero row.
+ * The logits are computed again, a piece of the vocabulary at a time; p - [v = target] is rounded to the inputs' dtype
+ * for the matrix cores, sums are fp32, one rounding at the end. Same limits; tokens >= 1. */
+long long qwen_cross_entropy_backward_workspace(int tokens, int vocab, int width, int want_hidden, int want_weight);
+int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const void* hidden,
+                                long long hidden_stride, const void* weight, long long weight_stride,
+                                const void* targets, int target_bits, int tokens, int vocab, int width, int dtype,
+                                long long ignore_index, const float* lse, void* grad_hidden, void* grad_weight,
+                                void* workspace, long long workspace_bytes, hipStream_t stream);
+
+/* Rows of x ([rows][stride], QWEN_F16 or QWEN_BF16) to 8-bit integers: scale[r] = max |x_r| / 127
+ * (fp32), q[r][c] = 127 x / max |x_r| to the nearest integer, ties to even (int8 [rows][width]). A row
+ * of zeros has scale 0; a row that holds an infinity or a NaN has scale NaN and zeros. width: a multiple
+ * of 16; stride: a multiple of 8, at least width; x and q 16-byte aligned. */
+int qwen_quantize_rows(const void* x, long long stride, int rows, int width, int dtype, signed char* q, float* scale,
+                       hipStream_t stream);
+
+/* Matrix product in 8-bit integers: out[t][n] = a_scale[t] b_scale[n] sum_k a[t][k] b[n][k], with
+ * a int8 [tokens][width], b int8 [channels][width], out [tokens][channels] in out_dtype (QWEN_F16,
+ * QWEN_BF16 or QWEN_F32). The sum is exact; the scaling is fp32, rounded once to out_dtype. width: a multiple of 16,
+ * at most 65536; a, b and out 16-byte aligned. */
+int qwen_matmul_i8(const signed char* a, const float* a_scale, const signed char* b, const float* b_scale, void* out,
+                   int out_dtype, int tokens, int channels, int width, hipStream_t stream);
+
 /* Synchronizes the current device and returns the device-side error state of
  * the last launches: QWEN_OK, QWEN_ERR_TIMEOUT (a wait exceeded its deadline)
  * or QWEN_ERR_BAD_TOKEN (a forced id out of range); clears it and resets the

@@ -223,6 +223,56 @@ def _pack_layer_weights(layer_weights: list) -> torch.Tensor:
     return t_aligned
 
 
+class _HeadLoss(torch.autograd.Function):
+    """Cross entropy of every position against the head, and [sum, count] of the positions that count."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index):
+        loss, lse, total = qwen_megakernel_C.lm_head_cross_entropy_total(hidden, weight, targets, ignore_index)
+        ctx.save_for_backward(hidden, weight, targets, lse)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(total)
+        return loss, total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss, _):
+        hidden, weight, targets, lse = ctx.saved_tensors
+        grads = qwen_megakernel_C.lm_head_cross_entropy_backward(
+            grad_loss, hidden, weight, targets, lse, ctx.ignore_index, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return (*grads, None, None)
+
+
+class _MeanOfLosses(torch.autograd.Function):
+    """The losses' sum, or their mean over the positions that count, from the total that came with them."""
+
+    @staticmethod
+    def forward(ctx, loss, total, mean):
+        ctx.positions = loss.shape[0]
+        ctx.mean = mean
+        ctx.save_for_backward(total)
+        return total[0] / total[1] if mean else total[0].clone()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (total,) = ctx.saved_tensors
+        grad = grad / total[1] if ctx.mean else grad
+        return grad.expand(ctx.positions), None, None
+
+
+def lm_head_loss(hidden, weight, targets, ignore_index: int = -100, reduction: str = "mean"):
+    """Softmax cross entropy of hidden rows [n, width] against a head's rows [vocabulary, width] without keeping the
+    logits, with gradients for both (fp16 or bf16; the loss is fp32). ``targets``: [n] int64 or int32, those equal
+    to ``ignore_index`` do not count. ``reduction``: "mean" over the positions that count (NaN if none does, as
+    0 / 0), "sum" or "none". fp16 gradients of a mean over many positions are small numbers: scale the loss, as
+    in any fp16 training."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
+    loss, total = _HeadLoss.apply(hidden, weight, targets, ignore_index)
+    return loss if reduction == "none" else _MeanOfLosses.apply(loss, total, reduction == "mean")
+
+
 class Decoder:
     """Stateful decoder over the MI355X decode engine (reference lines 205-382)."""
 

@@ -1,7 +1,8 @@
 """Build recipe for the engine (run from anywhere: ``python qwen0.6b_amd/build.py``).
 
 Produces, next to this file:
-  libqwen_megakernel.so                  the HIP kernels + C-ABI (hipcc, gfx950)
+  libqwen_megakernel.so                  the HIP kernels + C-ABI (hipcc, gfx950): the engine
+                                         (megakernel.hip) and the head's operators (head_ops.hip)
   qwen_megakernel_C<ext-suffix>          the pybind11 module over that C-ABI
   layout_check                           host-side exhaustive index checker (run here)
 
@@ -10,8 +11,8 @@ All HIP code is compiled with ``-Xclang -target-feature -Xclang -packed-fp32-ops
 compiler passes; the x86 host pass prints "'-packed-fp32-ops' is not a
 recognized feature for this target (ignoring feature)", the gfx950 device pass
 applies it. ``audit_device_code`` enforces the result on every build: it reads
-the gfx950 code object out of the built library, disassembles it and fails the
-build if it holds a packed fp32 add, multiply or fma, or any use of ``m0`` other
+the gfx950 code objects out of the built library, disassembles them and fails the
+build if they hold a packed fp32 add, multiply or fma, or any use of ``m0`` other
 than the ``s_mov_b32 m0`` that directly precedes each LDS-DMA load (the one
 inline-asm sequence that sets it; hipcc warns about that clobber).
 """
@@ -30,6 +31,7 @@ CSRC = os.path.join(HERE, "csrc")
 INC = os.path.join(REPO, "include")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
+SOURCES = ["megakernel.hip", "head_ops.hip"]
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # SimplifyCFG's common-code sinking merges the per-stage-type stores into the
 # compute waves' weight prefetch buffer into one store through a phi of
@@ -47,28 +49,31 @@ def _run(cmd):
 def build_kernels():
     out = os.path.join(HERE, "libqwen_megakernel.so")
     _run([HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared", f"-I{INC}", f"-I{CSRC}",
-          *NO_PACKED_FP32, *NO_SINK, os.path.join(CSRC, "megakernel.hip"), "-o", out])
+          *NO_PACKED_FP32, *NO_SINK, *[os.path.join(CSRC, f) for f in SOURCES], "-o", out])
     audit_device_code(out)
     return out
 
 
-def device_code_object(lib):
-    """The gfx950 code object inside a hipcc-built shared library (an uncompressed
-    clang offload bundle: 24-byte magic, entry count, then offset/size/triple per entry)."""
+def device_code_objects(lib):
+    """The gfx950 code objects inside a hipcc-built shared library, one per source file
+    (uncompressed clang offload bundles: 24-byte magic, entry count, then offset/size/triple per entry)."""
     data = open(lib, "rb").read()
-    base = data.find(b"__CLANG_OFFLOAD_BUNDLE__")
-    if base < 0:
-        raise RuntimeError(f"{lib}: no offload bundle found")
-    (n,) = struct.unpack_from("<Q", data, base + 24)
-    o = base + 32
-    for _ in range(n):
-        off, size, tlen = struct.unpack_from("<QQQ", data, o)
-        o += 24
-        triple = data[o:o + tlen].decode()
-        o += tlen
-        if triple.endswith(ARCH):
-            return data[base + off:base + off + size]
-    raise RuntimeError(f"{lib}: no {ARCH} code object in the bundle")
+    magic, found = b"__CLANG_OFFLOAD_BUNDLE__", []
+    base = data.find(magic)
+    while base >= 0:
+        (n,) = struct.unpack_from("<Q", data, base + 24)
+        o = base + 32
+        for _ in range(n):
+            off, size, tlen = struct.unpack_from("<QQQ", data, o)
+            o += 24
+            triple = data[o:o + tlen].decode()
+            o += tlen
+            if triple.endswith(ARCH):
+                found.append(data[base + off:base + off + size])
+        base = data.find(magic, o)
+    if len(found) != len(SOURCES):
+        raise RuntimeError(f"{lib}: {len(found)} {ARCH} code objects, expected {len(SOURCES)}")
+    return found
 
 
 def audit_device_code(lib):
@@ -76,11 +81,13 @@ def audit_device_code(lib):
     objdump = os.path.join(os.path.dirname(os.path.realpath(HIPCC)), "..", "llvm", "bin", "llvm-objdump")
     if not os.path.exists(objdump):
         objdump = "/opt/rocm/llvm/bin/llvm-objdump"
+    dis = ""
     with tempfile.TemporaryDirectory() as td:
-        co = os.path.join(td, "kernel.co")
-        with open(co, "wb") as f:
-            f.write(device_code_object(lib))
-        dis = subprocess.run([objdump, "-d", f"--mcpu={ARCH}", co], check=True, capture_output=True, text=True).stdout
+        for code in device_code_objects(lib):
+            co = os.path.join(td, "kernel.co")
+            with open(co, "wb") as f:
+                f.write(code)
+            dis += subprocess.run([objdump, "-d", f"--mcpu={ARCH}", co], check=True, capture_output=True, text=True).stdout
     ins = [ln.split("//")[0].strip() for ln in dis.splitlines() if ln[:1] in ("\t", " ")]
     ins = [x for x in ins if x]
     packed = [x for x in ins if re.match(r"v_pk_(add|mul|fma)_f32\b", x)]

@@ -1,0 +1,831 @@
+// Operators of the head over many positions, for gfx950: the cross entropy of hidden rows against a
+// head's rows, its gradients, the rounding of rows to 8-bit integers and the product of such rows.
+// None of their kernels waits for another workgroup; they may run beside anything.
+#include <hip/hip_runtime.h>
+#include <cstdint>
+#include <type_traits>
+
+#include "qwen_megakernel.h"
+
+#include "head_gemm.inc"
+
+namespace hd {
+
+constexpr int CUS = 256;
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+
+// targets as the caller holds them: 32- or 64-bit integers
+struct Targets {
+  const void* p;
+  int wide;
+  long long ignore;
+  __device__ __forceinline__ long long operator[](int t) const {
+    return wide ? ((const long long*)p)[t] : (long long)((const int*)p)[t];
+  }
+};
+
+// ---- forward: running softmax statistics over the vocabulary ---------------------------
+
+// First workgroup whose share of `items` holds item x, of `grid` (run_product's deal)
+__host__ __device__ inline int owner(long x, long items, long grid) { return (int)(((x + 1) * grid - 1) / items); }
+
+// Each lane keeps, for each of its tokens, the maximum m of the logits it has seen (in units of log 2) and
+// the sum of 2^(logit log2(e) - m); at the end of a workgroup's rows for a token tile they go to `part`,
+// one slot per workgroup and row half. The logits themselves stay in the accumulators.
+template <class C>
+struct Stats {
+  f32x2* part;  // [slot][tokens]
+  float* tl;    // [tokens] target's logit
+  Targets targets;
+  int tokens, vocab, tiles_t, tiles_n;
+  float m[C::NJ], s[C::NJ];
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) {
+      m[j] = -INFINITY;
+      s[j] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool last, int lane, int wn, int wt) {
+    const int n0 = at.tn * C::BN + 32 * C::NI * wn + 4 * (lane >> 5);  // register (i, q, r): row n0 + 32 i + 8 q + r
+    const int t0 = at.tt * C::BT + 32 * C::NJ * wt + (lane & 31);
+    if (at.tn * C::BN + 32 * C::NI * (wn + 1) > vocab) {  // rows past the vocabulary add nothing
+#pragma unroll
+      for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (n0 + 32 * i + 8 * (k >> 2) + (k & 3) >= vocab)
+#pragma unroll
+            for (int j = 0; j < C::NJ; ++j) acc[i][j][k] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) {
+      const int t = t0 + 32 * j;
+      const long long y = t < tokens ? targets[t] : -1;
+      const long d = (long)(y - n0);
+      if (__any(y != targets.ignore && d >= 0 && d < 32 * C::NI)) {
+#pragma unroll
+        for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (t < tokens && d == 32 * i + 8 * (k >> 2) + (k & 3)) tl[t] = acc[i][j][k];
+      }
+      float top = acc[0][j][0];
+#pragma unroll
+      for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) top = fmaxf(top, acc[i][j][k]);
+      const float to = fmaxf(m[j], top * LOG2E);
+      // all logits so far -inf: measured from 0, the exponentials are 0 (from -inf they would be NaN)
+      const float ref = to == -INFINITY ? 0.f : to;
+      float sum = s[j] * __builtin_amdgcn_exp2f(m[j] - ref);
+#pragma unroll
+      for (int i = 0; i < C::NI; ++i) {
+        float part_sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 16; ++k) part_sum[k & 3] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][k], LOG2E, -ref));
+        sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+      }
+      m[j] = to;
+      s[j] = sum;
+    }
+    if (last || at.tn + 1 == tiles_n) {
+      const long items = (long)tiles_t * tiles_n;
+      const int slot = ((int)blockIdx.x - owner((long)at.tt * tiles_n, items, gridDim.x)) * C::WN + wn;
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) {
+        const float mo = __shfl_xor(m[j], 32), so = __shfl_xor(s[j], 32);
+        const float to = fmaxf(m[j], mo), ref = to == -INFINITY ? 0.f : to;
+        const float sum = s[j] * __builtin_amdgcn_exp2f(m[j] - ref) + so * __builtin_amdgcn_exp2f(mo - ref);
+        if (lane < 32 && t0 + 32 * j < tokens) part[(long)slot * tokens + t0 + 32 * j] = f32x2{to, sum};
+      }
+      reset();
+    }
+  }
+};
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1) head_stats_kernel(Product P, Stats<C> epi) {
+  __shared__ __align__(16) char ring[C::RING];
+  epi.reset();
+  run_product<C>(P, ring, epi);
+}
+
+// Joins the slots of each token: 32 tokens per workgroup, 8 lanes' worth of slots each
+constexpr int JT = 32, JS = 8;
+__global__ void __launch_bounds__(JT* JS) head_join_kernel(const f32x2* part, const float* tl, Targets targets, int tokens,
+                                                           int vocab, int bt, int tiles_t, int tiles_n, int grid, int wn,
+                                                           float* loss, float* lse) {
+  __shared__ f32x2 sm[JS][JT];
+  const int i = threadIdx.x % JT, g = threadIdx.x / JT, t = blockIdx.x * JT + i;
+  float m = -INFINITY, s = 0.f;
+  if (t < tokens) {
+    const int tt = t / bt;
+    const long items = (long)tiles_t * tiles_n, a = (long)tt * tiles_n;
+    const int slots = (owner(a + tiles_n - 1, items, grid) - owner(a, items, grid) + 1) * wn;
+    for (int k = g; k < slots; k += JS) {
+      const f32x2 v = part[(long)k * tokens + t];
+      const float to = fmaxf(m, v[0]), ref = to == -INFINITY ? 0.f : to;
+      s = s * __builtin_amdgcn_exp2f(m - ref) + v[1] * __builtin_amdgcn_exp2f(v[0] - ref);
+      m = to;
+    }
+  }
+  sm[g][i] = f32x2{m, s};
+  __syncthreads();
+  if (g != 0 || t >= tokens) return;
+#pragma unroll
+  for (int k = 1; k < JS; ++k) {
+    const f32x2 v = sm[k][i];
+    const float to = fmaxf(m, v[0]), ref = to == -INFINITY ? 0.f : to;
+    s = s * __builtin_amdgcn_exp2f(m - ref) + v[1] * __builtin_amdgcn_exp2f(v[0] - ref);
+    m = to;
+  }
+  const float l = (m + log2f(s)) * LN2;
+  const long long y = targets[t];
+  lse[t] = l;
+  // a target that is neither a row of the head nor ignore_index makes the loss NaN
+  loss[t] = y == targets.ignore ? 0.f : (y < 0 || y >= vocab ? NAN : l - tl[t]);
+}
+
+// sum of the losses and number of the positions that count, in a fixed order
+__global__ void __launch_bounds__(1024) head_total_kernel(const float* loss, Targets targets, int tokens, float* total) {
+  __shared__ float sm[16];
+  __shared__ int cn[16];
+  float s = 0.f;
+  int n = 0;
+  for (int t = threadIdx.x; t < tokens; t += 1024) {
+    s += loss[t];
+    n += targets[t] != targets.ignore;
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    s += __shfl_xor(s, d);
+    n += __shfl_xor(n, d);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sm[threadIdx.x >> 6] = s;
+    cn[threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 1; k < 16; ++k) {
+    s += sm[k];
+    n += cn[k];
+  }
+  total[0] = s;
+  total[1] = (float)n;
+}
+
+// ---- stores of a tile ------------------------------------------------------------------
+
+// A wave's accumulators to memory as numbers of type T, 16 bytes per lane along the rows, by way of 8 KB of
+// LDS of its own: straight from the accumulators a store instruction would touch 32 lines for 16 bytes
+// each. make(j, t, i, q, v) turns the 4 accumulators of rows n .. n + 3 (v, in place) into what is stored at
+// token t; tokens from t_end and rows from n_end on are not stored. With `add` the fp32 numbers in memory
+// are added.
+template <class C, class T>
+struct Stores {
+  static constexpr int NB = C::NI < 8 / (int)sizeof(T) ? C::NI : 8 / (int)sizeof(T);  // tiles of 32 rows staged at a time
+  static constexpr int PER = 16 / sizeof(T), CH = 32 * NB / PER;                      // numbers per 16 bytes, 16 bytes per token
+  static_assert(C::NI % NB == 0 && 32 * CH * 16 <= 8192, "a wave's staging area");
+
+  template <class Make>
+  static __device__ __forceinline__ void store(typename C::E::acc (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wn,
+                                               int wt, char* lds, T* out, long ld, int t_end, int n_end, bool add,
+                                               Make&& make) {
+    const bool whole = n_end % PER == 0;  // (and ld with it: 16-byte stores stay inside the row and aligned)
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) {
+      const int tw = at.tt * C::BT + 32 * (C::NJ * wt + j);  // the wave's first token
+      const int tl = lane & 31;
+#pragma unroll
+      for (int ib = 0; ib < C::NI; ib += NB) {
+        const int nw = at.tn * C::BN + 32 * (C::NI * wn + ib);  // and row
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = (float)acc[ib + i][j][4 * q + r];
+            make(j, tw + tl, nw + 32 * i + 8 * q + 4 * (lane >> 5), v);
+            if (sizeof(T) == 2) {
+              typedef T t4 __attribute__((ext_vector_type(4)));
+              const int c = 4 * i + q;
+              *(t4*)(lds + (tl * CH + (c ^ (tl & (CH - 1)))) * 16 + 8 * (lane >> 5)) =
+                  t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+            } else {
+              const int c = 8 * i + 2 * q + (lane >> 5);
+              *(f32x4*)(lds + (tl * CH + (c ^ (tl & (CH - 1)))) * 16) = f32x4{v[0], v[1], v[2], v[3]};
+            }
+          }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int p = 0; p < 32 * CH / 64; ++p) {
+          const int e = 64 * p + lane, t = e / CH, c = e % CH, n = nw + PER * c;
+          typedef T tp __attribute__((ext_vector_type(PER)));
+          tp x = *(const tp*)(lds + (t * CH + (c ^ (t & (CH - 1)))) * 16);
+          if (tw + t >= t_end || n >= n_end) continue;
+          T* dst = out + (long)(tw + t) * ld + n;
+          if (whole) {
+            if (sizeof(T) == 4 && add) x += *(const tp*)dst;
+            *(tp*)dst = x;
+          } else {
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+              if (n + k < n_end) dst[k] = x[k];
+          }
+        }
+        asm volatile("" ::: "memory");
+      }
+    }
+  }
+};
+
+// ---- gradients -------------------------------------------------------------------------
+
+// The softmax's gradient of one piece of the vocabulary, G[t][v] = (2^(logit log2(e) - lse) - [v is the target])
+// * SCALE, in the inputs' 16-bit type: the next products take it as a matrix operand. fp16's SCALE (a power of
+// two, taken back at the end) keeps probabilities from 2^-29 on at full precision; without it those of a vocabulary
+// of 151936 would be subnormal. Tokens that do not count, and v past the vocabulary, get zeros.
+template <class E>
+constexpr float grad_scale() { return sizeof(typename E::elem) == 2 && std::is_same<E, Half>::value ? 32768.f : 1.f; }
+
+template <class C>
+struct Softgrad {
+  typedef typename C::E::elem T;
+  T* out;  // [tokens_pad][ld]
+  long ld;
+  const float* lse;
+  Targets targets;
+  int tokens, tokens_pad, v0, rows, rows_pad;  // the piece: vocabulary rows v0 .. v0 + rows - 1
+  char* lds;
+  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+    float l2[C::NJ];
+    long y[C::NJ];
+    bool counts[C::NJ];
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) {
+      const int t = at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31);
+      const long long target = t < tokens ? targets[t] : targets.ignore;
+      counts[j] = t < tokens && target != targets.ignore;
+      y[j] = (long)target - v0;
+      l2[j] = counts[j] ? lse[t] * LOG2E : 0.f;
+    }
+    Stores<C, T>::store(acc, at, lane, wn, wt, lds, out, ld, tokens_pad, rows_pad, false,
+                        [&](int j, int, int n, float (&v)[4]) {
+#pragma unroll
+                          for (int r = 0; r < 4; ++r) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(v[r], LOG2E, -l2[j]));
+                            const float g = (n + r == y[j] ? p - 1.f : p) * grad_scale<typename C::E>();
+                            v[r] = counts[j] && n + r < rows ? g : 0.f;
+                          }
+                        });
+  }
+};
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1) head_softgrad_kernel(Product P, Softgrad<C> epi) {
+  __shared__ __align__(16) char ring[C::RING];
+  __shared__ __align__(16) char stage[C::WAVES * 8192];
+  epi.lds = stage + (threadIdx.x >> 6) * 8192;
+  run_product<C>(P, ring, epi);
+}
+
+// Partial sums of grad_hidden, one [tokens][width] array per split, over the pieces one after the other
+template <class C>
+struct Partials {
+  float* out;
+  int tokens, width;
+  bool add;
+  char* lds;
+  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+    Stores<C, float>::store(acc, at, lane, wn, wt, lds, out + (long)at.split * tokens * width, width, tokens, width, add,
+                            [](int, int, int, float (&)[4]) {});
+  }
+};
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1) head_partials_kernel(Product P, Partials<C> epi) {
+  __shared__ __align__(16) char ring[C::RING];
+  __shared__ __align__(16) char stage[C::WAVES * 8192];
+  epi.lds = stage + (threadIdx.x >> 6) * 8192;
+  run_product<C>(P, ring, epi);
+}
+
+// grad_hidden: the splits' sums in order, times the position's upstream gradient
+template <class T>
+__global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part, int splits, int tokens, int width,
+                                                               Targets targets, const float* grad, long grad_stride,
+                                                               float unscale, T* out) {
+  const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 8, n = (long)tokens * width;
+  if (e >= n) return;
+  const int t = (int)(e / width);
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+  if (targets[t] != targets.ignore) {
+    for (int s = 0; s < splits; ++s) {
+      a += *(const f32x4*)(part + s * n + e);
+      b += *(const f32x4*)(part + s * n + e + 4);
+    }
+    const float g = grad[t * grad_stride] * unscale;
+    a *= g;
+    b *= g;
+  }
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  *(t8*)(out + e) = t8{(T)a[0], (T)a[1], (T)a[2], (T)a[3], (T)b[0], (T)b[1], (T)b[2], (T)b[3]};
+}
+
+// max |upstream gradient| of the positions that count
+__global__ void __launch_bounds__(1024) head_grad_max_kernel(const float* grad, long stride, Targets targets, int tokens,
+                                                             float* out) {
+  __shared__ float sm[16];
+  float m = 0.f;
+  for (int t = threadIdx.x; t < tokens; t += 1024)
+    if (targets[t] != targets.ignore) m = fmaxf(m, fabsf(grad[t * stride]));
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 1; k < 16; ++k) m = fmaxf(m, sm[k]);
+  *out = m;
+}
+
+// The hidden rows as grad_weight's product takes them: each times its upstream gradient over the largest one
+// (1, and no rounding, where all positions weigh the same), zeros for positions that do not count and
+// up to a whole number of K steps
+template <class T>
+__global__ void __launch_bounds__(256) head_weighted_rows_kernel(const T* hidden, long ld, Targets targets, const float* grad,
+                                                                 long grad_stride, const float* top, int tokens,
+                                                                 int tokens_pad, int width, T* out) {
+  const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (e >= (long)tokens_pad * width) return;
+  const int t = (int)(e / width), c = (int)(e % width);
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  t8 v;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = (T)0.f;
+  if (t < tokens && targets[t] != targets.ignore) {
+    const float m = *top, g = m == 0.f ? 0.f : grad[t * grad_stride] / m;
+    const t8 h = *(const t8*)(hidden + t * ld + c);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = (T)((float)h[k] * g);
+  }
+  *(t8*)(out + e) = v;
+}
+
+// grad_weight's rows of a piece
+template <class C>
+struct WeightGrad {
+  typedef typename C::E::elem T;
+  T* out;  // [rows][width]
+  const float* top;
+  int rows, width;
+  char* lds;
+  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+    const float f = *top * (1.f / grad_scale<typename C::E>());
+    Stores<C, T>::store(acc, at, lane, wn, wt, lds, out, width, rows, width, false, [&](int, int, int, float (&v)[4]) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] *= f;
+    });
+  }
+};
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1) head_weight_grad_kernel(Product P, WeightGrad<C> epi) {
+  __shared__ __align__(16) char ring[C::RING];
+  __shared__ __align__(16) char stage[C::WAVES * 8192];
+  epi.lds = stage + (threadIdx.x >> 6) * 8192;
+  run_product<C>(P, ring, epi);
+}
+
+// ---- 8-bit integers --------------------------------------------------------------------
+
+template <class C, class T>
+struct Dequant {
+  T* out;  // [tokens][rows]
+  const float *xs, *ws;
+  int tokens, rows;
+  char* lds;
+  __device__ __forceinline__ void tile(i32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+    float sx[C::NJ];
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) sx[j] = xs[min(at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31), tokens - 1)];
+    Stores<C, T>::store(acc, at, lane, wn, wt, lds, out, rows, tokens, rows, false, [&](int j, int, int n, float (&v)[4]) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] *= sx[j] * ws[min(n + r, rows - 1)];
+    });
+  }
+};
+template <class C, class T>
+__global__ void __launch_bounds__(C::THREADS, 1) matmul_i8_kernel(Product P, Dequant<C, T> epi) {
+  __shared__ __align__(16) char ring[C::RING];
+  __shared__ __align__(16) char stage[C::WAVES * 8192];
+  epi.lds = stage + (threadIdx.x >> 6) * 8192;
+  run_product<C>(P, ring, epi);
+}
+
+// Rows to 8-bit integers: scale = max |x| / 127, q = 127 x / max |x| rounded to the nearest integer, ties to even.
+// x has at most 11 significant bits, so 127 x is exact in fp32, and where 127 x / max |x| is not
+// k + 1/2 itself it differs from it by more than 2^-18 of its size: the fp32 division rounds to the same
+// integer as the exact quotient. A row of zeros gets scale 0; one with an infinity or a NaN scale NaN and
+// zeros, so that what is computed from it is NaN. One wave per row.
+template <class T>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long ld, int rows, int width, signed char* q,
+                                                            float* scale) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  const T* p = x + row * ld;
+  signed char* out = q + (long)row * width;
+  float top = 0.f;
+  bool bad = false;
+  for (int c = 8 * lane; c < width; c += 512) {
+    const t8 v = *(const t8*)(p + c);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float a = fabsf((float)v[k]);
+      bad |= !(a < INFINITY);
+      top = fmaxf(top, a);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  bad = __any(bad);
+  if (lane == 0) scale[row] = bad ? NAN : top / 127.f;
+  // (bf16: 127 x could pass fp32's range; a power of two leaves every quotient as it is)
+  const float f = top > 0x1p100f ? 0x1p-20f : 1.f, d = bad || top == 0.f ? INFINITY : top * f;
+  for (int c = 8 * lane; c < width; c += 512) {
+    const t8 v = *(const t8*)(p + c);
+    unsigned long long w = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float y = bad ? 0.f : rintf((float)v[k] * f * 127.f / d);
+      w |= (unsigned long long)(unsigned char)(signed char)(int)y << (8 * k);
+    }
+    *(unsigned long long*)(out + c) = w;
+  }
+}
+
+// ---- the engine's final norm over many rows --------------------------------------------
+
+// fp16(x / rms * gain) of fp32 rows of 1024, one wave per row
+__global__ void __launch_bounds__(256) norm_rows_kernel(const float* x, const _Float16* gain, int rows, _Float16* out) {
+  constexpr int H = 1024;
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  f32x4 v[4];
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[k] = *(const f32x4*)(x + (long)row * H + 8 * lane + 512 * (k >> 1) + 4 * (k & 1));
+    s += (v[k][0] * v[k][0] + v[k][1] * v[k][1]) + (v[k][2] * v[k][2] + v[k][3] * v[k][3]);
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+  const float r = rsqrtf(s * (1.f / H) + 1e-6f);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c = 8 * lane + 512 * k;
+    const f16x8 g = *(const f16x8*)(gain + c);
+    f16x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (_Float16)(v[2 * k + (e >> 2)][e & 3] * r * (float)g[e]);
+    *(f16x8*)(out + (long)row * H + c) = y;
+  }
+}
+
+// ====================================================================================
+// host side
+
+namespace {
+
+int launch(const void* kernel, long grid, int threads, void** args, hipStream_t stream) {
+  if (grid <= 0 || grid > 0x7fffffffL) return QWEN_ERR_ARG;
+  return hipLaunchKernel(kernel, dim3((unsigned)grid), dim3(threads), args, 0, stream) == hipSuccess ? QWEN_OK : QWEN_ERR_LAUNCH;
+}
+template <class P, class E>
+int launch_product(void (*kernel)(P, E), long grid, int threads, P product, E epi, hipStream_t stream) {
+  void* args[] = {&product, &epi};
+  return launch((const void*)kernel, grid, threads, args, stream);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+long round_up(long x, long m) { return (x + m - 1) / m * m; }
+
+template <class E, int LW = ROWS, int LX = ROWS>
+using Tile = Config<E, 128, 128, 2, 2, 3, LW, LX>;
+
+// a product's tiles over [tokens][rows]
+template <class C>
+Product make_product(Operand x, Operand w, int steps) {
+  Product P;
+  P.x = x;
+  P.w = w;
+  P.tiles_t = (x.n + C::BT - 1) / C::BT;
+  P.tiles_n = (w.n + C::BN - 1) / C::BN;
+  P.steps = steps;
+  P.splits = 1;
+  P.split_steps = steps;
+  return P;
+}
+long grid_of(const Product& P) {
+  const long items = (long)P.splits * P.tiles_t * P.tiles_n;
+  return items < CUS ? items : CUS;
+}
+int k_steps(long bytes) { return (int)((bytes + STEP - 1) / STEP); }
+
+struct Head {
+  const void* hidden;
+  long hidden_ld;
+  const void* weight;
+  long weight_ld;
+  Targets targets;
+  int tokens, vocab, width;
+};
+
+constexpr long MAX_ROW_BYTES = 4L << 20;  // a tile's offsets stay below 2^31
+constexpr int MAX_TOKENS = 1 << 20, MAX_VOCAB = 1 << 24;
+
+int check_head(const Head& h, int target_bits, int dtype) {
+  if (h.tokens < 0 || h.tokens > MAX_TOKENS || h.vocab < 1 || h.vocab > MAX_VOCAB || h.width < 8 || h.width % 8 != 0)
+    return QWEN_ERR_ARG;
+  if (dtype != QWEN_F16 && dtype != QWEN_BF16) return QWEN_ERR_ARG;
+  if (target_bits != 32 && target_bits != 64) return QWEN_ERR_ARG;
+  if (h.hidden_ld < h.width || h.weight_ld < h.width || h.hidden_ld % 8 != 0 || h.weight_ld % 8 != 0 ||
+      2 * h.hidden_ld > MAX_ROW_BYTES || 2 * h.weight_ld > MAX_ROW_BYTES)
+    return QWEN_ERR_ARG;
+  if (h.tokens > 0 && (!h.hidden || !h.targets.p || !aligned16(h.hidden) || ((uintptr_t)h.targets.p & (target_bits / 8 - 1)) != 0))
+    return QWEN_ERR_ARG;
+  if (!h.weight || !aligned16(h.weight)) return QWEN_ERR_ARG;
+  return QWEN_OK;
+}
+
+Operand rows_of(const void* p, long ld, int n, int width) { return Operand{(const char*)p, 2 * ld, n, 2 * width}; }
+
+struct ForwardPlan {
+  Product P;
+  long grid;
+  int wn, slots;
+};
+template <class C>
+ForwardPlan forward_plan(const Head& h) {
+  ForwardPlan f;
+  f.P = make_product<C>(rows_of(h.hidden, h.hidden_ld, h.tokens, h.width), rows_of(h.weight, h.weight_ld, h.vocab, h.width),
+                        k_steps(2L * h.width));
+  f.grid = grid_of(f.P);
+  f.wn = C::WN;
+  f.slots = 0;
+  const long items = (long)f.P.tiles_t * f.P.tiles_n;
+  for (long t = 0; t < f.P.tiles_t; ++t) {
+    const int n = owner((t + 1) * f.P.tiles_n - 1, items, f.grid) - owner(t * f.P.tiles_n, items, f.grid) + 1;
+    if (n > f.slots) f.slots = n;
+  }
+  f.slots *= C::WN;
+  return f;
+}
+template <class C>
+long forward_bytes(const Head& h) {
+  const ForwardPlan f = forward_plan<C>(h);
+  return round_up(8L * f.slots * h.tokens, 256) + round_up(4L * h.tokens, 256);
+}
+
+template <class C>
+int forward(const Head& h, float* loss, float* lse, float* total, char* ws, long ws_bytes, hipStream_t stream) {
+  if (ws_bytes < forward_bytes<C>(h)) return QWEN_ERR_ARG;
+  const ForwardPlan f = forward_plan<C>(h);
+  Stats<C> epi;
+  epi.part = (f32x2*)ws;
+  epi.tl = (float*)(ws + round_up(8L * f.slots * h.tokens, 256));
+  epi.targets = h.targets;
+  epi.tokens = h.tokens;
+  epi.vocab = h.vocab;
+  epi.tiles_t = f.P.tiles_t;
+  epi.tiles_n = f.P.tiles_n;
+  int rc = launch_product(head_stats_kernel<C>, f.grid, C::THREADS, f.P, epi, stream);
+  if (rc != QWEN_OK) return rc;
+  const f32x2* part = epi.part;
+  const float* tl = epi.tl;
+  Targets targets = h.targets;
+  int tokens = h.tokens, vocab = h.vocab, bt = C::BT, tt = f.P.tiles_t, tn = f.P.tiles_n, grid = (int)f.grid, wn = f.wn;
+  void* join[] = {&part, &tl, &targets, &tokens, &vocab, &bt, &tt, &tn, &grid, &wn, &loss, &lse};
+  rc = launch((const void*)head_join_kernel, (h.tokens + JT - 1) / JT, JT * JS, join, stream);
+  if (rc != QWEN_OK || !total) return rc;
+  void* sum[] = {&loss, &targets, &tokens, &total};
+  return launch((const void*)head_total_kernel, 1, 1024, sum, stream);
+}
+
+// ---- backward: pieces of the vocabulary
+
+struct BackwardPlan {
+  int tokens_pad;   // K of grad_weight's product
+  int rows;         // vocabulary rows per piece (a multiple of 256)
+  int splits, split_steps;  // of grad_hidden's product
+  long g, weighted, partial, top, bytes;  // places in the workspace
+};
+template <class E>
+BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
+  typedef Tile<E, COLS, ROWS> CH;
+  BackwardPlan b;
+  b.tokens_pad = (int)round_up(h.tokens, 64);
+  // the gradient of the logits is kept for a piece of the vocabulary: 128 MB, half of the 256 MB cache before HBM
+  constexpr long PIECE = 64L << 20;
+  const long rows = PIECE / b.tokens_pad / 256 * 256, all = round_up(h.vocab, 256);
+  b.rows = (int)(rows < 256 ? 256 : rows > all ? all : rows);
+  const long tiles = (long)((h.tokens + CH::BT - 1) / CH::BT) * ((h.width + CH::BN - 1) / CH::BN);
+  const int steps = (int)(round_up(b.rows < h.vocab ? b.rows : h.vocab, 64) / 64);  // of the first piece; no other has more
+  long s = CUS / tiles;
+  b.splits = (int)(s < 1 ? 1 : s > steps ? steps : s);
+  b.split_steps = (steps + b.splits - 1) / b.splits;
+  b.splits = (steps + b.split_steps - 1) / b.split_steps;
+  long at = 0;
+  auto take = [&](long bytes) {
+    const long p = at;
+    at += round_up(bytes, 256);
+    return p;
+  };
+  b.top = take(4);
+  b.g = take(2L * b.tokens_pad * b.rows);
+  b.weighted = take(want_weight ? 2L * b.tokens_pad * h.width : 0);
+  b.partial = take(want_hidden ? 4L * b.splits * h.tokens * h.width : 0);
+  b.bytes = at;
+  return b;
+}
+
+template <class E>
+int backward(const Head& h, const float* grad, long grad_stride, const float* lse, void* grad_hidden, void* grad_weight,
+             char* ws, long ws_bytes, hipStream_t stream) {
+  typedef typename E::elem T;
+  typedef Tile<E> CG;
+  typedef Tile<E, COLS, ROWS> CH;
+  typedef Tile<E, COLS, COLS> CW;
+  const BackwardPlan b = backward_plan<E>(h, grad_hidden, grad_weight);
+  if (ws_bytes < b.bytes) return QWEN_ERR_ARG;
+  T* g = (T*)(ws + b.g);
+  T* weighted = (T*)(ws + b.weighted);
+  float* partial = (float*)(ws + b.partial);
+  float* top = (float*)(ws + b.top);
+  Targets targets = h.targets;
+  int tokens = h.tokens, tokens_pad = b.tokens_pad, width = h.width;
+  int rc = QWEN_OK;
+  if (grad_weight) {
+    void* a[] = {&grad, &grad_stride, &targets, &tokens, &top};
+    if ((rc = launch((const void*)head_grad_max_kernel, 1, 1024, a, stream)) != QWEN_OK) return rc;
+    const T* hidden = (const T*)h.hidden;
+    long ld = h.hidden_ld;
+    void* c[] = {&hidden, &ld, &targets, &grad, &grad_stride, &top, &tokens, &tokens_pad, &width, &weighted};
+    rc = launch((const void*)head_weighted_rows_kernel<T>, ((long)tokens_pad * width / 8 + 255) / 256, 256, c, stream);
+    if (rc != QWEN_OK) return rc;
+  }
+  for (int v0 = 0; v0 < h.vocab; v0 += b.rows) {
+    const int rows = h.vocab - v0 < b.rows ? h.vocab - v0 : b.rows, rows_pad = (int)round_up(rows, 64);
+    const char* w = (const char*)h.weight + 2 * (long)v0 * h.weight_ld;
+    {
+      Product P = make_product<CG>(rows_of(h.hidden, h.hidden_ld, tokens, width), rows_of(w, h.weight_ld, rows, width),
+                                   k_steps(2L * width));
+      Softgrad<CG> e;
+      e.out = g;
+      e.ld = b.rows;
+      e.lse = lse;
+      e.targets = targets;
+      e.tokens = tokens;
+      e.tokens_pad = tokens_pad;
+      e.v0 = v0;
+      e.rows = rows;
+      e.rows_pad = rows_pad;
+      if ((rc = launch_product(head_softgrad_kernel<CG>, grid_of(P), CG::THREADS, P, e, stream)) != QWEN_OK) return rc;
+    }
+    if (grad_hidden) {
+      Operand x = {(const char*)g, 2L * b.rows, tokens, 2 * rows_pad};
+      Operand wt = {w, 2 * h.weight_ld, width, rows};
+      Product P = make_product<CH>(x, wt, rows_pad / 64);
+      P.split_steps = b.split_steps;
+      P.splits = (P.steps + P.split_steps - 1) / P.split_steps;
+      Partials<CH> e;
+      e.out = partial;
+      e.tokens = tokens;
+      e.width = width;
+      e.add = v0 > 0;
+      if ((rc = launch_product(head_partials_kernel<CH>, grid_of(P), CH::THREADS, P, e, stream)) != QWEN_OK) return rc;
+    }
+    if (grad_weight) {
+      Operand x = {(const char*)g, 2L * b.rows, rows_pad, tokens_pad};
+      Operand wt = {(const char*)weighted, 2L * width, width, tokens_pad};
+      Product P = make_product<CW>(x, wt, tokens_pad / 64);
+      WeightGrad<CW> e;
+      e.out = (T*)grad_weight + (long)v0 * width;
+      e.top = top;
+      e.rows = rows;
+      e.width = width;
+      if ((rc = launch_product(head_weight_grad_kernel<CW>, grid_of(P), CW::THREADS, P, e, stream)) != QWEN_OK) return rc;
+    }
+  }
+  if (grad_hidden) {
+    int splits = b.splits;
+    float unscale = 1.f / grad_scale<E>();
+    void* a[] = {&partial, &splits, &tokens, &width, &targets, &grad, &grad_stride, &unscale, &grad_hidden};
+    rc = launch((const void*)head_grad_hidden_kernel<T>, ((long)tokens * width / 8 + 255) / 256, 256, a, stream);
+  }
+  return rc;
+}
+
+}  // namespace
+}  // namespace hd
+
+using namespace hd;
+
+extern "C" long long qwen_cross_entropy_workspace(int tokens, int vocab, int width) {
+  if (tokens < 1 || tokens > MAX_TOKENS || vocab < 1 || vocab > MAX_VOCAB || width < 8) return 0;
+  Head h = {nullptr, 0, nullptr, 0, {}, tokens, vocab, width};
+  return forward_bytes<Tile<Half>>(h);
+}
+
+extern "C" int qwen_cross_entropy(const void* hidden, long long hidden_stride, const void* weight, long long weight_stride,
+                                  const void* targets, int target_bits, int tokens, int vocab, int width, int dtype,
+                                  long long ignore_index, float* loss, float* lse, float* total, void* workspace,
+                                  long long workspace_bytes, hipStream_t stream) {
+  const Head h = {hidden, (long)hidden_stride, weight, (long)weight_stride, {targets, target_bits == 64, ignore_index},
+                  tokens, vocab, width};
+  const int rc = check_head(h, target_bits, dtype);
+  if (rc != QWEN_OK) return rc;
+  if (tokens == 0) return QWEN_OK;
+  if (!loss || !lse || !workspace || !aligned16(workspace)) return QWEN_ERR_ARG;
+  char* ws = (char*)workspace;
+  return dtype == QWEN_F16 ? forward<Tile<Half>>(h, loss, lse, total, ws, workspace_bytes, stream)
+                           : forward<Tile<Bfloat>>(h, loss, lse, total, ws, workspace_bytes, stream);
+}
+
+extern "C" long long qwen_cross_entropy_backward_workspace(int tokens, int vocab, int width, int want_hidden, int want_weight) {
+  if (tokens < 1 || tokens > MAX_TOKENS || vocab < 1 || vocab > MAX_VOCAB || width < 8) return 0;
+  Head h = {nullptr, 0, nullptr, 0, {}, tokens, vocab, width};
+  return backward_plan<Half>(h, want_hidden != 0, want_weight != 0).bytes;
+}
+
+extern "C" int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const void* hidden,
+                                           long long hidden_stride, const void* weight, long long weight_stride,
+                                           const void* targets, int target_bits, int tokens, int vocab, int width,
+                                           int dtype, long long ignore_index, const float* lse, void* grad_hidden,
+                                           void* grad_weight, void* workspace, long long workspace_bytes,
+                                           hipStream_t stream) {
+  const Head h = {hidden, (long)hidden_stride, weight, (long)weight_stride, {targets, target_bits == 64, ignore_index},
+                  tokens, vocab, width};
+  const int rc = check_head(h, target_bits, dtype);
+  if (rc != QWEN_OK) return rc;
+  if (tokens < 1 || !grad_loss || grad_stride < 0 || !lse || (!grad_hidden && !grad_weight) || !aligned16(grad_hidden) ||
+      !aligned16(grad_weight) || !workspace || !aligned16(workspace))
+    return QWEN_ERR_ARG;
+  char* ws = (char*)workspace;
+  return dtype == QWEN_F16
+             ? backward<Half>(h, grad_loss, (long)grad_stride, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream)
+             : backward<Bfloat>(h, grad_loss, (long)grad_stride, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream);
+}
+
+extern "C" int qwen_quantize_rows(const void* x, long long stride, int rows, int width, int dtype, signed char* q,
+                                  float* scale, hipStream_t stream) {
+  if (rows < 0 || width < 16 || width % 16 != 0 || stride < width || stride % 8 != 0 || (dtype != QWEN_F16 && dtype != QWEN_BF16))
+    return QWEN_ERR_ARG;
+  if (rows == 0) return QWEN_OK;
+  if (!x || !q || !scale || !aligned16(x) || !aligned16(q)) return QWEN_ERR_ARG;
+  long ld = (long)stride;
+  void* args[] = {&x, &ld, &rows, &width, &q, &scale};
+  return launch(dtype == QWEN_F16 ? (const void*)quantize_rows_kernel<_Float16> : (const void*)quantize_rows_kernel<__bf16>,
+                ((long)rows + 3) / 4, 256, args, stream);
+}
+
+namespace hd {
+namespace {
+template <class T>
+int product_i8(const signed char* a, const float* as, const signed char* b, const float* bs, void* out, int tokens,
+               int channels, int width, hipStream_t stream) {
+  typedef Tile<Int8> C;
+  Product P = make_product<C>(Operand{(const char*)a, width, tokens, width}, Operand{(const char*)b, width, channels, width},
+                              k_steps(width));
+  Dequant<C, T> e;
+  e.out = (T*)out;
+  e.xs = as;
+  e.ws = bs;
+  e.tokens = tokens;
+  e.rows = channels;
+  return launch_product(matmul_i8_kernel<C, T>, grid_of(P), C::THREADS, P, e, stream);
+}
+}  // namespace
+
+// rows of the engine's residual stream through its final norm (called by qwen_prefill_hidden)
+int norm_rows(const float* x, const void* gain, int rows, void* out, hipStream_t stream) {
+  const _Float16* g = (const _Float16*)gain;
+  _Float16* o = (_Float16*)out;
+  void* args[] = {&x, &g, &rows, &o};
+  return launch((const void*)norm_rows_kernel, ((long)rows + 3) / 4, 256, args, stream);
+}
+}  // namespace hd
+
+extern "C" int qwen_matmul_i8(const signed char* a, const float* a_scale, const signed char* b, const float* b_scale,
+                              void* out, int out_dtype, int tokens, int channels, int width, hipStream_t stream) {
+  // 65536 products of 8-bit numbers stay within 2^30
+  if (tokens < 0 || channels < 0 || width < 16 || width % 16 != 0 || width > 65536) return QWEN_ERR_ARG;
+  if (out_dtype != QWEN_F16 && out_dtype != QWEN_BF16 && out_dtype != QWEN_F32) return QWEN_ERR_ARG;
+  if (tokens == 0 || channels == 0) return QWEN_OK;
+  if (!a || !a_scale || !b || !b_scale || !out || !aligned16(a) || !aligned16(b) || !aligned16(out)) return QWEN_ERR_ARG;
+  if (out_dtype == QWEN_F16) return product_i8<_Float16>(a, a_scale, b, b_scale, out, tokens, channels, width, stream);
+  if (out_dtype == QWEN_BF16) return product_i8<__bf16>(a, a_scale, b, b_scale, out, tokens, channels, width, stream);
+  return product_i8<float>(a, a_scale, b, b_scale, out, tokens, channels, width, stream);
+}

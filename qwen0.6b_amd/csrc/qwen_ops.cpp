@@ -309,6 +309,153 @@ torch::Tensor mlp_block(torch::Tensor x, torch::Tensor post_norm, torch::Tensor 
   return y;
 }
 
+// ---- the head over many positions
+
+int dtype_code(c10::ScalarType t, const char* name, bool f32 = false) {
+  if (t == torch::kHalf) return QWEN_F16;
+  if (t == torch::kBFloat16) return QWEN_BF16;
+  TORCH_CHECK(f32 && t == torch::kFloat, name, " has dtype ", c10::toString(t), ", expected ",
+              f32 ? "float16, bfloat16 or float32" : "float16 or bfloat16");
+  return QWEN_F32;
+}
+
+// a matrix whose rows are contiguous (and may lie further apart than their length); its row stride
+int64_t check_rows(const torch::Tensor& t, const char* name, int64_t multiple) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
+  TORCH_CHECK(t.dim() == 2, name, " has ", t.dim(), " dimensions, expected 2");
+  TORCH_CHECK(t.size(0) < (1LL << 31) && t.size(1) < (1LL << 31), name, " is too large");
+  TORCH_CHECK(t.size(1) > 0 && t.size(1) % multiple == 0, name, " has rows of ", t.size(1), ", expected a multiple of ", multiple);
+  if (t.size(0) == 0) return t.size(1);
+  TORCH_CHECK(t.stride(1) == 1, name, " must have contiguous rows");
+  const int64_t ld = t.size(0) == 1 ? t.size(1) : t.stride(0);  // (one row: its stride means nothing)
+  TORCH_CHECK(ld >= t.size(1) && ld % 8 == 0, name, " has row stride ", ld, ", expected a multiple of 8 and at least ", t.size(1));
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must be 16-byte aligned");
+  return ld;
+}
+
+struct HeadArgs {
+  int64_t hidden_ld, weight_ld;
+  int dtype, target_bits, tokens, vocab, width;
+  torch::Tensor targets;
+};
+HeadArgs check_head(const torch::Tensor& hidden, const torch::Tensor& weight, const torch::Tensor& targets) {
+  HeadArgs a;
+  a.dtype = dtype_code(hidden.scalar_type(), "hidden");
+  TORCH_CHECK(weight.scalar_type() == hidden.scalar_type(), "weight has dtype ", c10::toString(weight.scalar_type()),
+              ", expected hidden's, ", c10::toString(hidden.scalar_type()));
+  a.hidden_ld = check_rows(hidden, "hidden", 8);
+  a.weight_ld = check_rows(weight, "weight", 8);
+  TORCH_CHECK(weight.size(0) > 0, "weight has no rows");
+  TORCH_CHECK(weight.size(1) == hidden.size(1), "weight has rows of ", weight.size(1), ", hidden of ", hidden.size(1));
+  TORCH_CHECK(targets.is_cuda() && targets.dim() == 1 && targets.size(0) == hidden.size(0), "targets must be a GPU tensor of ",
+              hidden.size(0), " entries");
+  TORCH_CHECK(targets.scalar_type() == torch::kLong || targets.scalar_type() == torch::kInt,
+              "targets must be int64 or int32, not ", c10::toString(targets.scalar_type()));
+  TORCH_CHECK(weight.device() == hidden.device() && targets.device() == hidden.device(),
+              "hidden, weight and targets must be on one device");
+  a.targets = targets.contiguous();
+  a.target_bits = targets.scalar_type() == torch::kLong ? 64 : 32;
+  a.tokens = (int)hidden.size(0);
+  a.vocab = (int)weight.size(0);
+  a.width = (int)hidden.size(1);
+  return a;
+}
+torch::Tensor workspace_of(int64_t bytes, const torch::Tensor& like) {
+  return torch::empty({bytes}, torch::dtype(torch::kUInt8).device(like.device()));
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> cross_entropy(const torch::Tensor& hidden, const torch::Tensor& weight,
+                                                                      const torch::Tensor& targets, int64_t ignore_index,
+                                                                      bool want_total) {
+  const c10::DeviceGuard guard(hidden.device());
+  const HeadArgs a = check_head(hidden, weight, targets);
+  const auto f32 = torch::dtype(torch::kFloat).device(hidden.device());
+  auto loss = torch::empty({a.tokens}, f32), lse = torch::empty({a.tokens}, f32);
+  torch::Tensor total;
+  if (want_total) total = a.tokens ? torch::empty({2}, f32) : torch::zeros({2}, f32);
+  if (a.tokens == 0) return {loss, lse, total};
+  const auto ws = workspace_of(qwen_cross_entropy_workspace(a.tokens, a.vocab, a.width), hidden);
+  check_rc(qwen_cross_entropy(hidden.data_ptr(), a.hidden_ld, weight.data_ptr(), a.weight_ld, a.targets.data_ptr(),
+                              a.target_bits, a.tokens, a.vocab, a.width, a.dtype, ignore_index, loss.data_ptr<float>(),
+                              lse.data_ptr<float>(), want_total ? total.data_ptr<float>() : nullptr, ws.data_ptr(),
+                              ws.numel(), stream_of(hidden)),
+           "lm_head_cross_entropy");
+  return {loss, lse, total};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> lm_head_cross_entropy(torch::Tensor hidden, torch::Tensor weight,
+                                                               torch::Tensor targets, int64_t ignore_index) {
+  auto r = cross_entropy(hidden, weight, targets, ignore_index, false);
+  return {std::get<0>(r), std::get<1>(r)};
+}
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> lm_head_cross_entropy_total(torch::Tensor hidden, torch::Tensor weight,
+                                                                                    torch::Tensor targets,
+                                                                                    int64_t ignore_index) {
+  return cross_entropy(hidden, weight, targets, ignore_index, true);
+}
+
+std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> lm_head_cross_entropy_backward(
+    torch::Tensor grad_loss, torch::Tensor hidden, torch::Tensor weight, torch::Tensor targets, torch::Tensor lse,
+    int64_t ignore_index, bool need_hidden, bool need_weight) {
+  const c10::DeviceGuard guard(hidden.device());
+  const HeadArgs a = check_head(hidden, weight, targets);
+  TORCH_CHECK(grad_loss.is_cuda() && grad_loss.scalar_type() == torch::kFloat && grad_loss.dim() == 1 &&
+                  grad_loss.size(0) == a.tokens && grad_loss.device() == hidden.device(),
+              "grad_loss must be a float32 GPU tensor of ", a.tokens, " entries on hidden's device");
+  TORCH_CHECK(lse.device() == hidden.device() && lse.scalar_type() == torch::kFloat && lse.dim() == 1 && lse.size(0) == a.tokens &&
+                  lse.is_contiguous(),
+              "lse must be the contiguous float32 GPU tensor of ", a.tokens, " entries that the forward call gave");
+  c10::optional<torch::Tensor> gh, gw;
+  if (need_hidden) gh = torch::empty({a.tokens, a.width}, hidden.options());
+  if (need_weight) gw = a.tokens ? torch::empty({a.vocab, a.width}, weight.options()) : torch::zeros({a.vocab, a.width}, weight.options());
+  if (a.tokens == 0 || (!need_hidden && !need_weight)) return {gh, gw};
+  const auto ws = workspace_of(qwen_cross_entropy_backward_workspace(a.tokens, a.vocab, a.width, need_hidden, need_weight), hidden);
+  check_rc(qwen_cross_entropy_backward(grad_loss.data_ptr<float>(), a.tokens == 1 ? 0 : grad_loss.stride(0), hidden.data_ptr(),
+                                       a.hidden_ld, weight.data_ptr(), a.weight_ld, a.targets.data_ptr(), a.target_bits,
+                                       a.tokens, a.vocab, a.width, a.dtype, ignore_index, lse.data_ptr<float>(),
+                                       need_hidden ? gh->data_ptr() : nullptr, need_weight ? gw->data_ptr() : nullptr,
+                                       ws.data_ptr(), ws.numel(), stream_of(hidden)),
+           "lm_head_cross_entropy_backward");
+  return {gh, gw};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> quantize_rows(torch::Tensor x) {
+  const c10::DeviceGuard guard(x.device());
+  const int dtype = dtype_code(x.scalar_type(), "x");
+  const int64_t ld = check_rows(x, "x", 16);
+  auto q = torch::empty({x.size(0), x.size(1)}, torch::dtype(torch::kChar).device(x.device()));
+  auto scale = torch::empty({x.size(0)}, torch::dtype(torch::kFloat).device(x.device()));
+  check_rc(qwen_quantize_rows(x.data_ptr(), ld, (int)x.size(0), (int)x.size(1), dtype,
+                              reinterpret_cast<signed char*>(q.data_ptr()), scale.data_ptr<float>(), stream_of(x)),
+           "quantize_rows");
+  return {q, scale};
+}
+
+torch::Tensor matmul_i8(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
+                        c10::ScalarType out_dtype) {
+  const c10::DeviceGuard guard(a.device());
+  const int dtype = dtype_code(out_dtype, "out_dtype", true);
+  const torch::Tensor* q[2] = {&a, &b};
+  const torch::Tensor* s[2] = {&a_scale, &b_scale};
+  const char* name[2][2] = {{"a", "a_scale"}, {"b", "b_scale"}};
+  for (int k = 0; k < 2; ++k) {
+    TORCH_CHECK(q[k]->scalar_type() == torch::kChar, name[k][0], " must be int8");
+    check_rows(*q[k], name[k][0], 16);
+    TORCH_CHECK(q[k]->is_contiguous(), name[k][0], " must be contiguous");
+    TORCH_CHECK(s[k]->dim() == 1 && s[k]->size(0) == q[k]->size(0), name[k][1], " must have one entry for each row of ", name[k][0]);
+    check_dev(*s[k], name[k][1], torch::kFloat);
+    TORCH_CHECK(q[k]->device() == a.device() && s[k]->device() == a.device(), "a, b and their scales must be on one device");
+  }
+  TORCH_CHECK(b.size(1) == a.size(1), "b has rows of ", b.size(1), ", a of ", a.size(1));
+  TORCH_CHECK(a.size(1) <= 65536, "rows of ", a.size(1), " are longer than 65536");
+  auto out = torch::empty({a.size(0), b.size(0)}, torch::dtype(out_dtype).device(a.device()));
+  check_rc(qwen_matmul_i8(reinterpret_cast<const signed char*>(a.data_ptr()), a_scale.data_ptr<float>(),
+                          reinterpret_cast<const signed char*>(b.data_ptr()), b_scale.data_ptr<float>(), out.data_ptr(), dtype,
+                          (int)a.size(0), (int)b.size(0), (int)a.size(1), stream_of(a)),
+           "matmul_i8");
+  return out;
+}
+
 int last_error() { return qwen_last_error(); }
 
 void set_trace(c10::optional<torch::Tensor> buf, int token) {
@@ -352,6 +499,20 @@ PYBIND11_MODULE(qwen_megakernel_C, m) {
         pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("temperature"), pybind11::arg("top_k"),
         pybind11::arg("top_p"), pybind11::arg("seed"), pybind11::arg("position"),
         pybind11::arg("logits_out") = pybind11::none());
+  m.def("lm_head_cross_entropy", &lm_head_cross_entropy,
+        "cross entropy of hidden rows against the head's rows, without keeping the logits -> (loss, lse)",
+        pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("ignore_index") = -100);
+  m.def("lm_head_cross_entropy_total", &lm_head_cross_entropy_total,
+        "lm_head_cross_entropy, and [sum of the losses, positions that count]", pybind11::arg("hidden"),
+        pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("ignore_index") = -100);
+  m.def("lm_head_cross_entropy_backward", &lm_head_cross_entropy_backward,
+        "its gradients -> (grad_hidden, grad_weight), None for one that is not needed", pybind11::arg("grad_loss"),
+        pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("lse"),
+        pybind11::arg("ignore_index") = -100, pybind11::arg("need_hidden") = true, pybind11::arg("need_weight") = true);
+  m.def("quantize_rows", &quantize_rows, "rows to 8-bit integers with a scale each -> (q, scale)", pybind11::arg("x"));
+  m.def("matmul_i8", &matmul_i8, "product of 8-bit rows: out[t, n] = a_scale[t] b_scale[n] sum_k a[t, k] b[n, k]",
+        pybind11::arg("a"), pybind11::arg("a_scale"), pybind11::arg("b"), pybind11::arg("b_scale"),
+        pybind11::arg("out_dtype") = torch::kHalf);
   m.def("mlp_block", &mlp_block, "isolated RMSNorm + SwiGLU MLP + residual");
   m.def("prefill_timestamps", &prefill_timestamps, "wall-clock ticks (100 MHz) at the start and at every grid "
         "barrier of the last prefill: start, embedding, then QKV / attention / o_proj / gate-up / down per layer");
