@@ -275,7 +275,7 @@ int qwen_cross_entropy(const void* hidden, long long hidden_stride, const void* 
  * 0: one number for all positions)
  *   grad_hidden[t] = g_t sum_v (p_tv - [v = target_t]) w_v     ([tokens][width])
  *   grad_weight[v] = sum_t g_t (p_tv - [v = target_t]) h_t     ([vocab][width])
- * in the inputs' dtype; either may be null. lse is what qwen_cross_entropy gave for the same inputs.
+ * in the inputs' dtype; either may be null. loss and lse are what qwen_cross_entropy gave for the same inputs.
  * Positions that do not count take no part (their hidden rows may hold anything) and get a zero row.
  * The logits are computed again, a piece of the vocabulary at a time; p - [v = target] is rounded to the inputs' dtype
  * for the matrix cores, sums are fp32, one rounding at the end. Same limits; tokens >= 1. */
@@ -283,8 +283,8 @@ long long qwen_cross_entropy_backward_workspace(int tokens, int vocab, int width
 int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const void* hidden,
                                 long long hidden_stride, const void* weight, long long weight_stride,
                                 const void* targets, int target_bits, int tokens, int vocab, int width, int dtype,
-                                long long ignore_index, const float* lse, void* grad_hidden, void* grad_weight,
-                                void* workspace, long long workspace_bytes, hipStream_t stream);
+                                long long ignore_index, const float* loss, const float* lse, void* grad_hidden,
+                                void* grad_weight, void* workspace, long long workspace_bytes, hipStream_t stream);
 
 /* Rows of x ([rows][stride], QWEN_F16 or QWEN_BF16) to 8-bit integers: scale[r] = max |x_r| / 127
  * (fp32), q[r][c] = 127 x / max |x_r| to the nearest integer, ties to even (int8 [rows][width]). A row

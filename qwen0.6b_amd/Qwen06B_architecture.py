@@ -229,7 +229,7 @@ class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index):
         loss, lse, total = qwen_megakernel_C.lm_head_cross_entropy_total(hidden, weight, targets, ignore_index)
-        ctx.save_for_backward(hidden, weight, targets, lse)
+        ctx.save_for_backward(hidden, weight, targets, loss, lse)
         ctx.ignore_index = ignore_index
         ctx.mark_non_differentiable(total)
         return loss, total
@@ -237,9 +237,9 @@ class _HeadLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss, _):
-        hidden, weight, targets, lse = ctx.saved_tensors
+        hidden, weight, targets, loss, lse = ctx.saved_tensors
         grads = qwen_megakernel_C.lm_head_cross_entropy_backward(
-            grad_loss, hidden, weight, targets, lse, ctx.ignore_index, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+            grad_loss, hidden, weight, targets, loss, lse, ctx.ignore_index, *ctx.needs_input_grad[:2])
         return (*grads, None, None)
 
 

@@ -29,9 +29,27 @@ struct Targets {
 // First workgroup whose share of `items` holds item x, of `grid` (run_product's deal)
 __host__ __device__ inline int owner(long x, long items, long grid) { return (int)(((x + 1) * grid - 1) / items); }
 
+// Rows past the end of the head: logits of -inf, whose exponentials are 0
+template <class C>
+__device__ __forceinline__ void mask_rows(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wn, int rows) {
+  const int n0 = at.tn * C::BN + 32 * C::NI * wn;
+  if (n0 + 32 * C::NI <= rows) return;
+  int left = rows - n0 - 4 * (lane >> 5);
+#pragma unroll
+  for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        asm volatile("" : "+v"(left));  // (one comparison at a time: all masks at once do not fit the scalar registers)
+        acc[i][j][k] = 32 * i + 8 * (k >> 2) + (k & 3) >= left ? -INFINITY : acc[i][j][k];
+      }
+}
+
 // Each lane keeps, for each of its tokens, the maximum m of the logits it has seen (in units of log 2) and
-// the sum of 2^(logit log2(e) - m); at the end of a workgroup's rows for a token tile they go to `part`,
-// one slot per workgroup and row half. The logits themselves stay in the accumulators.
+// the sum of 2^(logit log2(e) - m), the target's own left out; at the end of a workgroup's rows for a
+// token tile they go to `part`, one slot per workgroup and row half. The logits themselves stay in the
+// accumulators.
 template <class C>
 struct Stats {
   f32x2* part;  // [slot][tokens]
@@ -50,26 +68,28 @@ struct Stats {
   __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool last, int lane, int wn, int wt) {
     const int n0 = at.tn * C::BN + 32 * C::NI * wn + 4 * (lane >> 5);  // register (i, q, r): row n0 + 32 i + 8 q + r
     const int t0 = at.tt * C::BT + 32 * C::NJ * wt + (lane & 31);
-    if (at.tn * C::BN + 32 * C::NI * (wn + 1) > vocab) {  // rows past the vocabulary add nothing
-#pragma unroll
-      for (int i = 0; i < C::NI; ++i)
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (n0 + 32 * i + 8 * (k >> 2) + (k & 3) >= vocab)
-#pragma unroll
-            for (int j = 0; j < C::NJ; ++j) acc[i][j][k] = -INFINITY;
-    }
+    mask_rows<C>(acc, at, lane, wn, vocab);
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) {
       const int t = t0 + 32 * j;
-      const long long y = t < tokens ? targets[t] : -1;
-      const long d = (long)(y - n0);
-      if (__any(y != targets.ignore && d >= 0 && d < 32 * C::NI)) {
+      const long long y = t < tokens ? targets[t] : targets.ignore;
+      const long long far = y - n0;
+      int d = y != targets.ignore && far >= 0 && far < 32 * C::NI ? (int)far : -1;
+      if (__any(d >= 0)) {
+        // the target's logit goes to `tl` and leaves the sum: see head_join_kernel
+        float x = 0.f;
+        bool here = false;
 #pragma unroll
         for (int i = 0; i < C::NI; ++i)
 #pragma unroll
-          for (int k = 0; k < 16; ++k)
-            if (t < tokens && d == 32 * i + 8 * (k >> 2) + (k & 3)) tl[t] = acc[i][j][k];
+          for (int k = 0; k < 16; ++k) {
+            asm volatile("" : "+v"(d));  // (one comparison at a time: 64 masks kept at once do not fit the scalar registers)
+            const bool hit = d == 32 * i + 8 * (k >> 2) + (k & 3);
+            x = hit ? acc[i][j][k] : x;
+            here |= hit;
+            acc[i][j][k] = hit ? -INFINITY : acc[i][j][k];
+          }
+        if (here) tl[t] = x;
       }
       float top = acc[0][j][0];
 #pragma unroll
@@ -141,11 +161,24 @@ __global__ void __launch_bounds__(JT* JS) head_join_kernel(const f32x2* part, co
     s = s * __builtin_amdgcn_exp2f(m - ref) + v[1] * __builtin_amdgcn_exp2f(v[0] - ref);
     m = to;
   }
-  const float l = (m + log2f(s)) * LN2;
   const long long y = targets[t];
-  lse[t] = l;
-  // a target that is neither a row of the head nor ignore_index makes the loss NaN
-  loss[t] = y == targets.ignore ? 0.f : (y < 0 || y >= vocab ? NAN : l - tl[t]);
+  if (y == targets.ignore || y < 0 || y >= vocab) {
+    lse[t] = (m + log2f(s)) * LN2;
+    loss[t] = y == targets.ignore ? 0.f : NAN;  // neither a row of the head nor ignore_index
+    return;
+  }
+  // With the sum S of the other rows' exponentials apart, the loss log(S + e^l) - l is log1p(S e^-l) where l is large:
+  // the loss of a target that the model is sure of is not the difference of two numbers that are nearly equal.
+  const float l = tl[t], d = fmaf(l, LOG2E, -m);  // the target's logit above the others' largest, in units of log 2
+  if (d > 0.f) {
+    const float x = log1pf(s * __builtin_amdgcn_exp2f(-d));
+    loss[t] = l == INFINITY ? NAN : x;
+    lse[t] = l + x;
+  } else {
+    const float all = s + __builtin_amdgcn_exp2f(d);  // (at least 1)
+    loss[t] = (log2f(all) - d) * LN2;
+    lse[t] = (m + log2f(all)) * LN2;
+  }
 }
 
 // sum of the losses and number of the positions that count, in a fixed order
@@ -179,16 +212,19 @@ __global__ void __launch_bounds__(1024) head_total_kernel(const float* loss, Tar
 
 // ---- stores of a tile ------------------------------------------------------------------
 
-// A wave's accumulators to memory as numbers of type T, 16 bytes per lane along the rows, by way of 8 KB of
+constexpr int STAGING = 32768;  // bytes of LDS, shared out among the waves
+
+// A wave's accumulators to memory as numbers of type T, 16 bytes per lane along the rows, by way of
 // LDS of its own: straight from the accumulators a store instruction would touch 32 lines for 16 bytes
 // each. make(j, t, i, q, v) turns the 4 accumulators of rows n .. n + 3 (v, in place) into what is stored at
 // token t; tokens from t_end and rows from n_end on are not stored. With `add` the fp32 numbers in memory
 // are added.
 template <class C, class T>
 struct Stores {
-  static constexpr int NB = C::NI < 8 / (int)sizeof(T) ? C::NI : 8 / (int)sizeof(T);  // tiles of 32 rows staged at a time
-  static constexpr int PER = 16 / sizeof(T), CH = 32 * NB / PER;                      // numbers per 16 bytes, 16 bytes per token
-  static_assert(C::NI % NB == 0 && 32 * CH * 16 <= 8192, "a wave's staging area");
+  static constexpr int FIT = STAGING / C::WAVES / 1024 / (int)sizeof(T);
+  static constexpr int NB = C::NI < FIT ? C::NI : FIT;            // tiles of 32 rows staged at a time
+  static constexpr int PER = 16 / sizeof(T), CH = 32 * NB / PER;  // numbers per 16 bytes, 16 bytes per token
+  static_assert(C::NI % NB == 0 && NB >= 1, "a wave's staging area");
 
   template <class Make>
   static __device__ __forceinline__ void store(typename C::E::acc (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wn,
@@ -257,29 +293,32 @@ struct Softgrad {
   typedef typename C::E::elem T;
   T* out;  // [tokens_pad][ld]
   long ld;
-  const float* lse;
+  const float *loss, *lse;
   Targets targets;
   int tokens, tokens_pad, v0, rows, rows_pad;  // the piece: vocabulary rows v0 .. v0 + rows - 1
   char* lds;
   __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
-    float l2[C::NJ];
-    long y[C::NJ];
+    float l2[C::NJ], own[C::NJ];
+    int y[C::NJ];
     bool counts[C::NJ];
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) {
       const int t = at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31);
       const long long target = t < tokens ? targets[t] : targets.ignore;
       counts[j] = t < tokens && target != targets.ignore;
-      y[j] = (long)target - v0;
+      const long long far = target - v0;
+      y[j] = far >= 0 && far < rows ? (int)far : -1;
       l2[j] = counts[j] ? lse[t] * LOG2E : 0.f;
+      own[j] = counts[j] ? expm1f(-loss[t]) : 0.f;  // the target's: p - 1, also where p is nearly 1
     }
+    mask_rows<C>(acc, at, lane, wn, rows);
     Stores<C, T>::store(acc, at, lane, wn, wt, lds, out, ld, tokens_pad, rows_pad, false,
                         [&](int j, int, int n, float (&v)[4]) {
 #pragma unroll
                           for (int r = 0; r < 4; ++r) {
                             const float p = __builtin_amdgcn_exp2f(fmaf(v[r], LOG2E, -l2[j]));
-                            const float g = (n + r == y[j] ? p - 1.f : p) * grad_scale<typename C::E>();
-                            v[r] = counts[j] && n + r < rows ? g : 0.f;
+                            const float g = (n + r == y[j] ? own[j] : p) * grad_scale<typename C::E>();
+                            v[r] = counts[j] ? g : 0.f;
                           }
                         });
   }
@@ -288,8 +327,8 @@ struct Softgrad {
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, 1) head_softgrad_kernel(Product P, Softgrad<C> epi) {
   __shared__ __align__(16) char ring[C::RING];
-  __shared__ __align__(16) char stage[C::WAVES * 8192];
-  epi.lds = stage + (threadIdx.x >> 6) * 8192;
+  __shared__ __align__(16) char stage[STAGING];
+  epi.lds = stage + (threadIdx.x >> 6) * (STAGING / C::WAVES);
   run_product<C>(P, ring, epi);
 }
 
@@ -308,8 +347,8 @@ struct Partials {
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, 1) head_partials_kernel(Product P, Partials<C> epi) {
   __shared__ __align__(16) char ring[C::RING];
-  __shared__ __align__(16) char stage[C::WAVES * 8192];
-  epi.lds = stage + (threadIdx.x >> 6) * 8192;
+  __shared__ __align__(16) char stage[STAGING];
+  epi.lds = stage + (threadIdx.x >> 6) * (STAGING / C::WAVES);
   run_product<C>(P, ring, epi);
 }
 
@@ -393,8 +432,8 @@ struct WeightGrad {
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, 1) head_weight_grad_kernel(Product P, WeightGrad<C> epi) {
   __shared__ __align__(16) char ring[C::RING];
-  __shared__ __align__(16) char stage[C::WAVES * 8192];
-  epi.lds = stage + (threadIdx.x >> 6) * 8192;
+  __shared__ __align__(16) char stage[STAGING];
+  epi.lds = stage + (threadIdx.x >> 6) * (STAGING / C::WAVES);
   run_product<C>(P, ring, epi);
 }
 
@@ -419,8 +458,8 @@ struct Dequant {
 template <class C, class T>
 __global__ void __launch_bounds__(C::THREADS, 1) matmul_i8_kernel(Product P, Dequant<C, T> epi) {
   __shared__ __align__(16) char ring[C::RING];
-  __shared__ __align__(16) char stage[C::WAVES * 8192];
-  epi.lds = stage + (threadIdx.x >> 6) * 8192;
+  __shared__ __align__(16) char stage[STAGING];
+  epi.lds = stage + (threadIdx.x >> 6) * (STAGING / C::WAVES);
   run_product<C>(P, ring, epi);
 }
 
@@ -513,7 +552,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 long round_up(long x, long m) { return (x + m - 1) / m * m; }
 
 template <class E, int LW = ROWS, int LX = ROWS>
-using Tile = Config<E, 128, 128, 2, 2, 3, LW, LX>;
+using Tile = Config<E, 256, 256, 2, 4, 2, LW, LX>;
 
 // a product's tiles over [tokens][rows]
 template <class C>
@@ -652,8 +691,8 @@ BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
 }
 
 template <class E>
-int backward(const Head& h, const float* grad, long grad_stride, const float* lse, void* grad_hidden, void* grad_weight,
-             char* ws, long ws_bytes, hipStream_t stream) {
+int backward(const Head& h, const float* grad, long grad_stride, const float* loss, const float* lse, void* grad_hidden,
+             void* grad_weight, char* ws, long ws_bytes, hipStream_t stream) {
   typedef typename E::elem T;
   typedef Tile<E> CG;
   typedef Tile<E, COLS, ROWS> CH;
@@ -685,6 +724,7 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* ls
       Softgrad<CG> e;
       e.out = g;
       e.ld = b.rows;
+      e.loss = loss;
       e.lse = lse;
       e.targets = targets;
       e.tokens = tokens;
@@ -763,20 +803,20 @@ extern "C" long long qwen_cross_entropy_backward_workspace(int tokens, int vocab
 extern "C" int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const void* hidden,
                                            long long hidden_stride, const void* weight, long long weight_stride,
                                            const void* targets, int target_bits, int tokens, int vocab, int width,
-                                           int dtype, long long ignore_index, const float* lse, void* grad_hidden,
-                                           void* grad_weight, void* workspace, long long workspace_bytes,
-                                           hipStream_t stream) {
+                                           int dtype, long long ignore_index, const float* loss, const float* lse,
+                                           void* grad_hidden, void* grad_weight, void* workspace,
+                                           long long workspace_bytes, hipStream_t stream) {
   const Head h = {hidden, (long)hidden_stride, weight, (long)weight_stride, {targets, target_bits == 64, ignore_index},
                   tokens, vocab, width};
   const int rc = check_head(h, target_bits, dtype);
   if (rc != QWEN_OK) return rc;
-  if (tokens < 1 || !grad_loss || grad_stride < 0 || !lse || (!grad_hidden && !grad_weight) || !aligned16(grad_hidden) ||
+  if (tokens < 1 || !grad_loss || grad_stride < 0 || !loss || !lse || (!grad_hidden && !grad_weight) || !aligned16(grad_hidden) ||
       !aligned16(grad_weight) || !workspace || !aligned16(workspace))
     return QWEN_ERR_ARG;
   char* ws = (char*)workspace;
   return dtype == QWEN_F16
-             ? backward<Half>(h, grad_loss, (long)grad_stride, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream)
-             : backward<Bfloat>(h, grad_loss, (long)grad_stride, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream);
+             ? backward<Half>(h, grad_loss, (long)grad_stride, loss, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream)
+             : backward<Bfloat>(h, grad_loss, (long)grad_stride, loss, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream);
 }
 
 extern "C" int qwen_quantize_rows(const void* x, long long stride, int rows, int width, int dtype, signed char* q,

@@ -395,16 +395,17 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> lm_head_cross_entropy_to
 }
 
 std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> lm_head_cross_entropy_backward(
-    torch::Tensor grad_loss, torch::Tensor hidden, torch::Tensor weight, torch::Tensor targets, torch::Tensor lse,
-    int64_t ignore_index, bool need_hidden, bool need_weight) {
+    torch::Tensor grad_loss, torch::Tensor hidden, torch::Tensor weight, torch::Tensor targets, torch::Tensor loss,
+    torch::Tensor lse, int64_t ignore_index, bool need_hidden, bool need_weight) {
   const c10::DeviceGuard guard(hidden.device());
   const HeadArgs a = check_head(hidden, weight, targets);
   TORCH_CHECK(grad_loss.is_cuda() && grad_loss.scalar_type() == torch::kFloat && grad_loss.dim() == 1 &&
                   grad_loss.size(0) == a.tokens && grad_loss.device() == hidden.device(),
               "grad_loss must be a float32 GPU tensor of ", a.tokens, " entries on hidden's device");
-  TORCH_CHECK(lse.device() == hidden.device() && lse.scalar_type() == torch::kFloat && lse.dim() == 1 && lse.size(0) == a.tokens &&
-                  lse.is_contiguous(),
-              "lse must be the contiguous float32 GPU tensor of ", a.tokens, " entries that the forward call gave");
+  for (const auto& t : {loss, lse})
+    TORCH_CHECK(t.device() == hidden.device() && t.scalar_type() == torch::kFloat && t.dim() == 1 && t.size(0) == a.tokens &&
+                    t.is_contiguous(),
+                "loss and lse must be the contiguous float32 GPU tensors of ", a.tokens, " entries that the forward call gave");
   c10::optional<torch::Tensor> gh, gw;
   if (need_hidden) gh = torch::empty({a.tokens, a.width}, hidden.options());
   if (need_weight) gw = a.tokens ? torch::empty({a.vocab, a.width}, weight.options()) : torch::zeros({a.vocab, a.width}, weight.options());
@@ -412,8 +413,8 @@ std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> lm_head_c
   const auto ws = workspace_of(qwen_cross_entropy_backward_workspace(a.tokens, a.vocab, a.width, need_hidden, need_weight), hidden);
   check_rc(qwen_cross_entropy_backward(grad_loss.data_ptr<float>(), a.tokens == 1 ? 0 : grad_loss.stride(0), hidden.data_ptr(),
                                        a.hidden_ld, weight.data_ptr(), a.weight_ld, a.targets.data_ptr(), a.target_bits,
-                                       a.tokens, a.vocab, a.width, a.dtype, ignore_index, lse.data_ptr<float>(),
-                                       need_hidden ? gh->data_ptr() : nullptr, need_weight ? gw->data_ptr() : nullptr,
+                                       a.tokens, a.vocab, a.width, a.dtype, ignore_index, loss.data_ptr<float>(),
+                                       lse.data_ptr<float>(), need_hidden ? gh->data_ptr() : nullptr, need_weight ? gw->data_ptr() : nullptr,
                                        ws.data_ptr(), ws.numel(), stream_of(hidden)),
            "lm_head_cross_entropy_backward");
   return {gh, gw};
@@ -507,7 +508,7 @@ PYBIND11_MODULE(qwen_megakernel_C, m) {
         pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("ignore_index") = -100);
   m.def("lm_head_cross_entropy_backward", &lm_head_cross_entropy_backward,
         "its gradients -> (grad_hidden, grad_weight), None for one that is not needed", pybind11::arg("grad_loss"),
-        pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("lse"),
+        pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("loss"), pybind11::arg("lse"),
         pybind11::arg("ignore_index") = -100, pybind11::arg("need_hidden") = true, pybind11::arg("need_weight") = true);
   m.def("quantize_rows", &quantize_rows, "rows to 8-bit integers with a scale each -> (q, scale)", pybind11::arg("x"));
   m.def("matmul_i8", &matmul_i8, "product of 8-bit rows: out[t, n] = a_scale[t] b_scale[n] sum_k a[t, k] b[n, k]",

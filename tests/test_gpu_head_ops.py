@@ -68,8 +68,8 @@ def check_forward(ext, h, w, y, ignore=IGNORE):
     return loss, lse
 
 
-def check_backward(ext, h, w, y, lse, g, ignore=IGNORE, need_hidden=True, need_weight=True):
-    gh, gw = ext.lm_head_cross_entropy_backward(g, h, w, y, lse, ignore, need_hidden, need_weight)
+def check_backward(ext, h, w, y, fwd, g, ignore=IGNORE, need_hidden=True, need_weight=True):
+    gh, gw = ext.lm_head_cross_entropy_backward(g, h, w, y, *fwd, ignore, need_hidden, need_weight)
     assert (gh is not None) == need_hidden and (gw is not None) == need_weight
     dt = h.dtype
     u = U[dt]
@@ -119,20 +119,20 @@ SIZES = [  # tokens, vocabulary, width: single ones, one less and one more than 
 @pytest.mark.parametrize("tokens,vocab,width", SIZES)
 def test_cross_entropy_and_gradients(ext, tokens, vocab, width, dtype):
     h, w, y = make(tokens, vocab, width, dtype, seed=tokens)
-    _, lse = check_forward(ext, h, w, y)
+    fwd = check_forward(ext, h, w, y)
     g = torch.rand(tokens, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) + 0.5
-    check_backward(ext, h, w, y, lse, g)
+    check_backward(ext, h, w, y, fwd, g)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_full_head(ext, dtype):
     h, w, y = make(130, 151936, 1024, dtype, seed=5)
-    _, lse = check_forward(ext, h, w, y)
-    check_backward(ext, h, w, y, lse, torch.full((130,), 8.0, device="cuda"))
+    fwd = check_forward(ext, h, w, y)
+    check_backward(ext, h, w, y, fwd, torch.full((130,), 8.0, device="cuda"))
 
 
 def test_several_pieces_of_the_vocabulary(ext):
     """More positions than let the whole vocabulary's gradient be kept at once."""
     h, w, y = make(4100, 40009, 64, torch.bfloat16, seed=6)
-    _, lse = check_forward(ext, h, w, y)
-    check_backward(ext, h, w, y, lse, torch.full((4100,), 0.25, device="cuda"))
+    fwd = check_forward(ext, h, w, y)
+    check_backward(ext, h, w, y, fwd, torch.full((4100,), 0.25, device="cuda"))
