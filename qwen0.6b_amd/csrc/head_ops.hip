@@ -46,12 +46,20 @@ __device__ __forceinline__ void mask_rows(f32x16 (&acc)[C::NI][C::NJ], const Cur
       }
 }
 
+// two running sums over disjoint rows into one
+__device__ __forceinline__ void join(float& m, float& s, float mo, float so) {
+  const float to = fmaxf(m, mo), ref = to == -INFINITY ? 0.f : to;
+  s = s * __builtin_amdgcn_exp2f(m - ref) + so * __builtin_amdgcn_exp2f(mo - ref);
+  m = to;
+}
+
 // Each lane keeps, for each of its tokens, the maximum m of the logits it has seen (in units of log 2) and
 // the sum of 2^(logit log2(e) - m), the target's own left out; at the end of a workgroup's rows for a
 // token tile they go to `part`, one slot per workgroup and row half. The logits themselves stay in the
 // accumulators.
 template <class C>
-struct Stats {
+struct Stats : FromZero<C> {
+  static constexpr int STORES = 0;
   f32x2* part;  // [slot][tokens]
   float* tl;    // [tokens] target's logit
   Targets targets;
@@ -65,7 +73,8 @@ struct Stats {
       s[j] = 0.f;
     }
   }
-  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool last, int lane, int wn, int wt) {
+  __device__ __forceinline__ bool tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool last, int lane, int wn, int wt) {
+    asm volatile("" : "+v"(lane));  // (as in Stores)
     const int n0 = at.tn * C::BN + 32 * C::NI * wn + 4 * (lane >> 5);  // register (i, q, r): row n0 + 32 i + 8 q + r
     const int t0 = at.tt * C::BT + 32 * C::NJ * wt + (lane & 31);
     mask_rows<C>(acc, at, lane, wn, vocab);
@@ -116,51 +125,47 @@ struct Stats {
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j) {
         const float mo = __shfl_xor(m[j], 32), so = __shfl_xor(s[j], 32);
-        const float to = fmaxf(m[j], mo), ref = to == -INFINITY ? 0.f : to;
-        const float sum = s[j] * __builtin_amdgcn_exp2f(m[j] - ref) + so * __builtin_amdgcn_exp2f(mo - ref);
-        if (lane < 32 && t0 + 32 * j < tokens) part[(long)slot * tokens + t0 + 32 * j] = f32x2{to, sum};
+        join(m[j], s[j], mo, so);
+        if (lane < 32 && t0 + 32 * j < tokens) part[(long)slot * tokens + t0 + 32 * j] = f32x2{m[j], s[j]};
       }
       reset();
     }
+    return false;
   }
 };
 
 template <class C>
-__global__ void __launch_bounds__(C::THREADS, 1) head_stats_kernel(Product P, Stats<C> epi) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_stats_kernel(Product P, Stats<C> epi) {
   __shared__ __align__(16) char ring[C::RING];
   epi.reset();
   run_product<C>(P, ring, epi);
 }
 
-// Joins the slots of each token: 32 tokens per workgroup, 8 lanes' worth of slots each
-constexpr int JT = 32, JS = 8;
+// Joins the slots of each token: 8 tokens per workgroup, 32 lanes' worth of slots each
+constexpr int JT = 8, JS = 32;
 __global__ void __launch_bounds__(JT* JS) head_join_kernel(const f32x2* part, const float* tl, Targets targets, int tokens,
                                                            int vocab, int bt, int tiles_t, int tiles_n, int grid, int wn,
                                                            float* loss, float* lse) {
-  __shared__ f32x2 sm[JS][JT];
+  __shared__ f32x2 sm[JS / 8][JT];
   const int i = threadIdx.x % JT, g = threadIdx.x / JT, t = blockIdx.x * JT + i;
   float m = -INFINITY, s = 0.f;
   if (t < tokens) {
     const int tt = t / bt;
     const long items = (long)tiles_t * tiles_n, a = (long)tt * tiles_n;
     const int slots = (owner(a + tiles_n - 1, items, grid) - owner(a, items, grid) + 1) * wn;
+#pragma unroll 4
     for (int k = g; k < slots; k += JS) {
       const f32x2 v = part[(long)k * tokens + t];
-      const float to = fmaxf(m, v[0]), ref = to == -INFINITY ? 0.f : to;
-      s = s * __builtin_amdgcn_exp2f(m - ref) + v[1] * __builtin_amdgcn_exp2f(v[0] - ref);
-      m = to;
+      join(m, s, v[0], v[1]);
     }
   }
-  sm[g][i] = f32x2{m, s};
+#pragma unroll
+  for (int d = JT; d < 64; d *= 2) join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
+  if ((threadIdx.x & 63) < JT) sm[threadIdx.x >> 6][i] = f32x2{m, s};
   __syncthreads();
   if (g != 0 || t >= tokens) return;
 #pragma unroll
-  for (int k = 1; k < JS; ++k) {
-    const f32x2 v = sm[k][i];
-    const float to = fmaxf(m, v[0]), ref = to == -INFINITY ? 0.f : to;
-    s = s * __builtin_amdgcn_exp2f(m - ref) + v[1] * __builtin_amdgcn_exp2f(v[0] - ref);
-    m = to;
-  }
+  for (int k = 1; k < JS / 8; ++k) join(m, s, sm[k][i][0], sm[k][i][1]);
   const long long y = targets[t];
   if (y == targets.ignore || y < 0 || y >= vocab) {
     lse[t] = (m + log2f(s)) * LN2;
@@ -212,32 +217,50 @@ __global__ void __launch_bounds__(1024) head_total_kernel(const float* loss, Tar
 
 // ---- stores of a tile ------------------------------------------------------------------
 
-constexpr int STAGING = 32768;  // bytes of LDS, shared out among the waves
-
-// A wave's accumulators to memory as numbers of type T, 16 bytes per lane along the rows, by way of
+// A wave's accumulators to memory as numbers of type T, 16 bytes per lane along the rows, by way of 4 KB of
 // LDS of its own: straight from the accumulators a store instruction would touch 32 lines for 16 bytes
-// each. make(j, t, i, q, v) turns the 4 accumulators of rows n .. n + 3 (v, in place) into what is stored at
-// token t; tokens from t_end and rows from n_end on are not stored. With `add` the fp32 numbers in memory
-// are added.
+// each. make(i, q, j, v) turns the 4 accumulators of rows 32 i + 8 q + 4 (lane / 32) .. + 3 of the wave's (v, in
+// place) into what is stored; patch(ib, j) may then change numbers in LDS, and last(j, token, x) changes the
+// 16 bytes that go out for one of the wave's 32 tokens. Tokens from t_end and rows from n_end on are not stored.
+// Returns whether exactly COUNT stores were sent (not where some lanes' are left out).
+// (The stores take a scalar base and a vector offset: with buffer stores that take a scalar offset of their own, now
+// and then 16 bytes of a tile were wrong.)
+struct Nothing {
+  __device__ void operator()(int, int) const {}
+  __device__ void operator()(int, int, u32x4&) const {}
+};
 template <class C, class T>
 struct Stores {
-  static constexpr int FIT = STAGING / C::WAVES / 1024 / (int)sizeof(T);
+  static constexpr int FIT = 4 / (int)sizeof(T);
   static constexpr int NB = C::NI < FIT ? C::NI : FIT;            // tiles of 32 rows staged at a time
   static constexpr int PER = 16 / sizeof(T), CH = 32 * NB / PER;  // numbers per 16 bytes, 16 bytes per token
   static_assert(C::NI % NB == 0 && NB >= 1, "a wave's staging area");
+  static constexpr int COUNT = C::NJ * (C::NI / NB) * (32 * CH / 64);
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  typedef T tp __attribute__((ext_vector_type(PER)));
+  // where the wave's LDS holds chunk c of token t
+  static __device__ __forceinline__ u32 place(int t, int c) { return (u32)(t * CH * 16 + ((c ^ (t & (CH - 1))) << 4)); }
 
-  template <class Make>
-  static __device__ __forceinline__ void store(typename C::E::acc (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wn,
-                                               int wt, char* lds, T* out, long ld, int t_end, int n_end, bool add,
-                                               Make&& make) {
-    const bool whole = n_end % PER == 0;  // (and ld with it: 16-byte stores stay inside the row and aligned)
+  template <class Make, class Patch, class Last>
+  static __device__ __forceinline__ bool store(typename C::E::acc (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wn,
+                                               int wt, char* lds, T* out, long ld, int t_end, int n_end, Make&& make,
+                                               Patch&& patch, Last&& last) {
+    // (what follows from `lane` is computed here, item by item, rather than kept in registers through the K loop)
+    asm volatile("" : "+v"(lane));
+    const bool whole = n_end % PER == 0 && ld % PER == 0 && ((size_t)out & 15) == 0;  // 16-byte stores are aligned and end with the row
+    const int t0 = at.tt * C::BT + 32 * C::NJ * wt, n0 = at.tn * C::BN + 32 * C::NI * wn;  // the wave's first token and row
+    const bool inner = whole && t0 + 32 * C::NJ <= t_end && n0 + 32 * C::NI <= n_end;
+    char* base = (char*)uniform((const char*)(out + (long)t0 * ld + n0));
+    const int tl = lane & 31;
+    const u32 to = place(tl, 0) + 8 * (sizeof(T) == 2 ? lane >> 5 : 0);  // (chunk c: to ^ 16 c)
+    // reading back, a lane has 16 bytes of token 64 / CH p + lane / CH
+    constexpr int TP = 64 / CH;
+    const int tr = lane / CH, cr = lane % CH;
+    const u32 off = (u32)(tr * (int)ld + PER * cr) * (u32)sizeof(T);
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) {
-      const int tw = at.tt * C::BT + 32 * (C::NJ * wt + j);  // the wave's first token
-      const int tl = lane & 31;
 #pragma unroll
       for (int ib = 0; ib < C::NI; ib += NB) {
-        const int nw = at.tn * C::BN + 32 * (C::NI * wn + ib);  // and row
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -245,37 +268,37 @@ struct Stores {
             float v[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] = (float)acc[ib + i][j][4 * q + r];
-            make(j, tw + tl, nw + 32 * i + 8 * q + 4 * (lane >> 5), v);
-            if (sizeof(T) == 2) {
-              typedef T t4 __attribute__((ext_vector_type(4)));
-              const int c = 4 * i + q;
-              *(t4*)(lds + (tl * CH + (c ^ (tl & (CH - 1)))) * 16 + 8 * (lane >> 5)) =
-                  t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-            } else {
-              const int c = 8 * i + 2 * q + (lane >> 5);
-              *(f32x4*)(lds + (tl * CH + (c ^ (tl & (CH - 1)))) * 16) = f32x4{v[0], v[1], v[2], v[3]};
-            }
+            make(ib + i, q, j, v);
+            const u32 c = sizeof(T) == 2 ? 16 * (4 * i + q) : 16 * (8 * i + 2 * q + (lane >> 5));
+            *(t4*)(lds + (to ^ c)) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
           }
         asm volatile("" ::: "memory");
+        patch(ib, j);
+        asm volatile("" ::: "memory");
 #pragma unroll
-        for (int p = 0; p < 32 * CH / 64; ++p) {
-          const int e = 64 * p + lane, t = e / CH, c = e % CH, n = nw + PER * c;
-          typedef T tp __attribute__((ext_vector_type(PER)));
-          tp x = *(const tp*)(lds + (t * CH + (c ^ (t & (CH - 1)))) * 16);
-          if (tw + t >= t_end || n >= n_end) continue;
-          T* dst = out + (long)(tw + t) * ld + n;
-          if (whole) {
-            if (sizeof(T) == 4 && add) x += *(const tp*)dst;
-            *(tp*)dst = x;
-          } else {
+        for (int p = 0; p < 32 / TP; ++p) {
+          const int t = TP * p + tr;
+          u32x4 x = *(const u32x4*)(lds + place(t, cr));
+          last(j, t, x);
+          if (inner) {
+            *(u32x4*)(base + ((long)(32 * j + TP * p) * ld + 32 * ib) * (long)sizeof(T) + off) = x;
+          } else if (t0 + 32 * j + t < t_end && n0 + 32 * ib + PER * cr < n_end) {
+            const int n = n0 + 32 * ib + PER * cr;
+            T* dst = out + (long)(t0 + 32 * j + t) * ld + n;
+            if (n + PER <= n_end) {
+              __builtin_memcpy(dst, &x, 16);
+            } else {
+              const tp y = __builtin_bit_cast(tp, x);
 #pragma unroll
-            for (int k = 0; k < PER; ++k)
-              if (n + k < n_end) dst[k] = x[k];
+              for (int k = 0; k < PER; ++k)
+                if (n + k < n_end) dst[k] = y[k];
+            }
           }
         }
         asm volatile("" ::: "memory");
       }
     }
+    return inner;
   }
 };
 
@@ -289,89 +312,121 @@ template <class E>
 constexpr float grad_scale() { return sizeof(typename E::elem) == 2 && std::is_same<E, Half>::value ? 32768.f : 1.f; }
 
 template <class C>
-struct Softgrad {
+struct Softgrad : FromZero<C> {
   typedef typename C::E::elem T;
+  typedef Stores<C, T> St;
+  static constexpr int STORES = St::COUNT;
   T* out;  // [tokens_pad][ld]
   long ld;
   const float *loss, *lse;
   Targets targets;
   int tokens, tokens_pad, v0, rows, rows_pad;  // the piece: vocabulary rows v0 .. v0 + rows - 1
   char* lds;
-  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+  __device__ __forceinline__ bool tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+    constexpr float SCALE = grad_scale<typename C::E>();
     float l2[C::NJ], own[C::NJ];
-    int y[C::NJ];
-    bool counts[C::NJ];
+    int y[C::NJ];       // the target's row of the wave's, where it is one of them
+    u32 counts[C::NJ];  // a bit per token
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) {
       const int t = at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31);
       const long long target = t < tokens ? targets[t] : targets.ignore;
-      counts[j] = t < tokens && target != targets.ignore;
-      const long long far = target - v0;
-      y[j] = far >= 0 && far < rows ? (int)far : -1;
-      l2[j] = counts[j] ? lse[t] * LOG2E : 0.f;
-      own[j] = counts[j] ? expm1f(-loss[t]) : 0.f;  // the target's: p - 1, also where p is nearly 1
+      const bool c = t < tokens && target != targets.ignore;
+      counts[j] = (u32)__ballot(c);
+      const long long far = target - v0, row = far - (at.tn * C::BN + 32 * C::NI * wn);
+      y[j] = c && lane < 32 && far < rows && row >= 0 && row < 32 * C::NI ? (int)row : -1;
+      l2[j] = c ? fmaf(lse[t], LOG2E, -__builtin_log2f(SCALE)) : 0.f;
+      own[j] = c ? expm1f(-loss[t]) * SCALE : 0.f;  // the target's p - 1, also where p is nearly 1
     }
     mask_rows<C>(acc, at, lane, wn, rows);
-    Stores<C, T>::store(acc, at, lane, wn, wt, lds, out, ld, tokens_pad, rows_pad, false,
-                        [&](int j, int, int n, float (&v)[4]) {
+    return St::store(
+        acc, at, lane, wn, wt, lds, out, ld, tokens_pad, rows_pad,
+        [&](int, int, int j, float (&v)[4]) {
 #pragma unroll
-                          for (int r = 0; r < 4; ++r) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(v[r], LOG2E, -l2[j]));
-                            const float g = (n + r == y[j] ? own[j] : p) * grad_scale<typename C::E>();
-                            v[r] = counts[j] ? g : 0.f;
-                          }
-                        });
+          for (int r = 0; r < 4; ++r) v[r] = __builtin_amdgcn_exp2f(fmaf(v[r], LOG2E, -l2[j]));
+        },
+        [&](int ib, int j) {
+          const int n = y[j] - 32 * ib;
+          if (n >= 0 && n < 32 * St::NB) *(T*)(lds + St::place(lane & 31, n / St::PER) + (int)sizeof(T) * (n % St::PER)) = (T)own[j];
+        },
+        [&](int j, int t, u32x4& x) {
+          // (a mask: what a token that does not count holds may be NaN)
+          x &= (u32)__builtin_amdgcn_sbfe((int)counts[j], t, 1);
+        });
   }
 };
 
 template <class C>
-__global__ void __launch_bounds__(C::THREADS, 1) head_softgrad_kernel(Product P, Softgrad<C> epi) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_softgrad_kernel(Product P, Softgrad<C> epi) {
   __shared__ __align__(16) char ring[C::RING];
-  __shared__ __align__(16) char stage[STAGING];
-  epi.lds = stage + (threadIdx.x >> 6) * (STAGING / C::WAVES);
+  __shared__ __align__(16) char stage[C::STAGING];
+  epi.lds = stage + (threadIdx.x >> 6) * 4096;
   run_product<C>(P, ring, epi);
 }
 
-// Partial sums of grad_hidden, one [tokens][width] array per split, over the pieces one after the other
+// Partial sums of grad_hidden: the accumulators of each item as the lanes hold them (fp32, 16 bytes per lane, 1 KB
+// per wave and store), carried on from one piece of the vocabulary to the next
 template <class C>
 struct Partials {
-  float* out;
-  int tokens, width;
+  static constexpr int STORES = 0;
+  float* out;  // [item][wave][i][j][q][lane][4]
   bool add;
-  char* lds;
-  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
-    Stores<C, float>::store(acc, at, lane, wn, wt, lds, out + (long)at.split * tokens * width, width, tokens, width, add,
-                            [](int, int, int, float (&)[4]) {});
+  static __host__ __device__ __forceinline__ long place(long item, int wave, int i, int j) {
+    return ((item * C::WAVES + wave) * C::NI * C::NJ + i * C::NJ + j) * 1024;
+  }
+  __device__ __forceinline__ void begin(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wave) {
+    asm volatile("" : "+v"(lane));  // (as in Stores)
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v = {0.f, 0.f, 0.f, 0.f};
+          if (add) v = *(const f32x4*)(out + place(at.item, wave, i, j) + 256 * q + 4 * lane);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][4 * q + r] = v[r];
+        }
+  }
+  __device__ __forceinline__ bool tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+    asm volatile("" : "+v"(lane));
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *(f32x4*)(out + place(at.item, wt * C::WN + wn, i, j) + 256 * q + 4 * lane) =
+              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    return false;
   }
 };
 template <class C>
-__global__ void __launch_bounds__(C::THREADS, 1) head_partials_kernel(Product P, Partials<C> epi) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_partials_kernel(Product P, Partials<C> epi) {
   __shared__ __align__(16) char ring[C::RING];
-  __shared__ __align__(16) char stage[STAGING];
-  epi.lds = stage + (threadIdx.x >> 6) * (STAGING / C::WAVES);
   run_product<C>(P, ring, epi);
 }
 
-// grad_hidden: the splits' sums in order, times the position's upstream gradient
-template <class T>
-__global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part, int splits, int tokens, int width,
-                                                               Targets targets, const float* grad, long grad_stride,
-                                                               float unscale, T* out) {
-  const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 8, n = (long)tokens * width;
-  if (e >= n) return;
-  const int t = (int)(e / width);
-  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+// grad_hidden: the splits' sums in order, times the position's upstream gradient; a thread has 4 numbers of one row
+template <class C>
+__global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part, int splits, int tiles_t, int tiles_n,
+                                                               int tokens, int width, Targets targets, const float* grad,
+                                                               long grad_stride, float unscale, typename C::E::elem* out) {
+  typedef typename C::E::elem T;
+  constexpr int PER_TILE = C::BN * C::BT / 4;
+  const long e = (long)blockIdx.x * 256 + threadIdx.x;
+  const int tile = (int)(e / PER_TILE), o = (int)(e % PER_TILE);
+  const int wave = o / (C::NI * C::NJ * 256), ij = o / 256 % (C::NI * C::NJ), q = o / 64 % 4, lane = o % 64;
+  const int t = tile / tiles_n * C::BT + 32 * (C::NJ * (wave / C::WN) + ij % C::NJ) + (lane & 31);
+  const int n = tile % tiles_n * C::BN + 32 * (C::NI * (wave % C::WN) + ij / C::NJ) + 8 * q + 4 * (lane >> 5);
+  if (tile >= tiles_t * tiles_n || t >= tokens || n >= width) return;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
   if (targets[t] != targets.ignore) {
-    for (int s = 0; s < splits; ++s) {
-      a += *(const f32x4*)(part + s * n + e);
-      b += *(const f32x4*)(part + s * n + e + 4);
-    }
-    const float g = grad[t * grad_stride] * unscale;
-    a *= g;
-    b *= g;
+    for (int s = 0; s < splits; ++s) a += *(const f32x4*)(part + ((long)s * tiles_t * tiles_n * PER_TILE + e) * 4);
+    a *= grad[t * grad_stride] * unscale;
   }
-  typedef T t8 __attribute__((ext_vector_type(8)));
-  *(t8*)(out + e) = t8{(T)a[0], (T)a[1], (T)a[2], (T)a[3], (T)b[0], (T)b[1], (T)b[2], (T)b[3]};
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  *(t4*)(out + (long)t * width + n) = t4{(T)a[0], (T)a[1], (T)a[2], (T)a[3]};
 }
 
 // max |upstream gradient| of the positions that count
@@ -415,51 +470,74 @@ __global__ void __launch_bounds__(256) head_weighted_rows_kernel(const T* hidden
 
 // grad_weight's rows of a piece
 template <class C>
-struct WeightGrad {
+struct WeightGrad : FromZero<C> {
   typedef typename C::E::elem T;
+  static constexpr int STORES = Stores<C, T>::COUNT;
   T* out;  // [rows][width]
   const float* top;
   int rows, width;
   char* lds;
-  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+  __device__ __forceinline__ bool tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
     const float f = *top * (1.f / grad_scale<typename C::E>());
-    Stores<C, T>::store(acc, at, lane, wn, wt, lds, out, width, rows, width, false, [&](int, int, int, float (&v)[4]) {
+    return Stores<C, T>::store(
+        acc, at, lane, wn, wt, lds, out, width, rows, width,
+        [&](int, int, int, float (&v)[4]) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] *= f;
-    });
+          for (int r = 0; r < 4; ++r) v[r] *= f;
+        },
+        Nothing(), Nothing());
   }
 };
 template <class C>
-__global__ void __launch_bounds__(C::THREADS, 1) head_weight_grad_kernel(Product P, WeightGrad<C> epi) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_weight_grad_kernel(Product P, WeightGrad<C> epi) {
   __shared__ __align__(16) char ring[C::RING];
-  __shared__ __align__(16) char stage[STAGING];
-  epi.lds = stage + (threadIdx.x >> 6) * (STAGING / C::WAVES);
+  __shared__ __align__(16) char stage[C::STAGING];
+  epi.lds = stage + (threadIdx.x >> 6) * 4096;
   run_product<C>(P, ring, epi);
 }
 
 // ---- 8-bit integers --------------------------------------------------------------------
 
 template <class C, class T>
-struct Dequant {
+struct Dequant : FromZero<C> {
+  static constexpr int STORES = Stores<C, T>::COUNT;
   T* out;  // [tokens][rows]
   const float *xs, *ws;
   int tokens, rows;
   char* lds;
-  __device__ __forceinline__ void tile(i32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+  __device__ __forceinline__ bool tile(i32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+    const int n0 = at.tn * C::BN + 32 * C::NI * wn + 4 * (lane >> 5);
     float sx[C::NJ];
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) sx[j] = xs[min(at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31), tokens - 1)];
-    Stores<C, T>::store(acc, at, lane, wn, wt, lds, out, rows, tokens, rows, false, [&](int j, int, int n, float (&v)[4]) {
+    // the rows' scales, 4 together (the wave's rows may end before its tile does)
+    f32x4 sw[C::NI][4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] *= sx[j] * ws[min(n + r, rows - 1)];
-    });
+    for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + 32 * i + 8 * q;
+        if (at.tn * C::BN + 32 * (C::NI * wn + i + 1) <= rows) {
+          __builtin_memcpy(&sw[i][q], ws + n, 16);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sw[i][q][r] = ws[min(n + r, rows - 1)];
+        }
+      }
+    return Stores<C, T>::store(
+        acc, at, lane, wn, wt, lds, out, rows, tokens, rows,
+        [&](int i, int q, int j, float (&v)[4]) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] *= sx[j] * sw[i][q][r];
+        },
+        Nothing(), Nothing());
   }
 };
 template <class C, class T>
-__global__ void __launch_bounds__(C::THREADS, 1) matmul_i8_kernel(Product P, Dequant<C, T> epi) {
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) matmul_i8_kernel(Product P, Dequant<C, T> epi) {
   __shared__ __align__(16) char ring[C::RING];
-  __shared__ __align__(16) char stage[STAGING];
-  epi.lds = stage + (threadIdx.x >> 6) * (STAGING / C::WAVES);
+  __shared__ __align__(16) char stage[C::STAGING];
+  epi.lds = stage + (threadIdx.x >> 6) * 4096;
   run_product<C>(P, ring, epi);
 }
 
@@ -552,7 +630,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 long round_up(long x, long m) { return (x + m - 1) / m * m; }
 
 template <class E, int LW = ROWS, int LX = ROWS>
-using Tile = Config<E, 256, 256, 2, 4, 2, LW, LX>;
+using Tile = Config<E, 256, 256, 2, 4, 2, 1, LW, LX>;
 
 // a product's tiles over [tokens][rows]
 template <class C>
@@ -567,9 +645,10 @@ Product make_product(Operand x, Operand w, int steps) {
   P.split_steps = steps;
   return P;
 }
+template <class C>
 long grid_of(const Product& P) {
   const long items = (long)P.splits * P.tiles_t * P.tiles_n;
-  return items < CUS ? items : CUS;
+  return items < CUS * C::OCC ? items : CUS * C::OCC;
 }
 int k_steps(long bytes) { return (int)((bytes + STEP - 1) / STEP); }
 
@@ -611,7 +690,7 @@ ForwardPlan forward_plan(const Head& h) {
   ForwardPlan f;
   f.P = make_product<C>(rows_of(h.hidden, h.hidden_ld, h.tokens, h.width), rows_of(h.weight, h.weight_ld, h.vocab, h.width),
                         k_steps(2L * h.width));
-  f.grid = grid_of(f.P);
+  f.grid = grid_of<C>(f.P);
   f.wn = C::WN;
   f.slots = 0;
   const long items = (long)f.P.tiles_t * f.P.tiles_n;
@@ -685,7 +764,7 @@ BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
   b.top = take(4);
   b.g = take(2L * b.tokens_pad * b.rows);
   b.weighted = take(want_weight ? 2L * b.tokens_pad * h.width : 0);
-  b.partial = take(want_hidden ? 4L * b.splits * h.tokens * h.width : 0);
+  b.partial = take(want_hidden ? 4L * b.splits * tiles * CH::BN * CH::BT : 0);
   b.bytes = at;
   return b;
 }
@@ -732,7 +811,7 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* lo
       e.v0 = v0;
       e.rows = rows;
       e.rows_pad = rows_pad;
-      if ((rc = launch_product(head_softgrad_kernel<CG>, grid_of(P), CG::THREADS, P, e, stream)) != QWEN_OK) return rc;
+      if ((rc = launch_product(head_softgrad_kernel<CG>, grid_of<CG>(P), CG::THREADS, P, e, stream)) != QWEN_OK) return rc;
     }
     if (grad_hidden) {
       Operand x = {(const char*)g, 2L * b.rows, tokens, 2 * rows_pad};
@@ -742,10 +821,8 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* lo
       P.splits = (P.steps + P.split_steps - 1) / P.split_steps;
       Partials<CH> e;
       e.out = partial;
-      e.tokens = tokens;
-      e.width = width;
       e.add = v0 > 0;
-      if ((rc = launch_product(head_partials_kernel<CH>, grid_of(P), CH::THREADS, P, e, stream)) != QWEN_OK) return rc;
+      if ((rc = launch_product(head_partials_kernel<CH>, grid_of<CH>(P), CH::THREADS, P, e, stream)) != QWEN_OK) return rc;
     }
     if (grad_weight) {
       Operand x = {(const char*)g, 2L * b.rows, rows_pad, tokens_pad};
@@ -756,14 +833,14 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* lo
       e.top = top;
       e.rows = rows;
       e.width = width;
-      if ((rc = launch_product(head_weight_grad_kernel<CW>, grid_of(P), CW::THREADS, P, e, stream)) != QWEN_OK) return rc;
+      if ((rc = launch_product(head_weight_grad_kernel<CW>, grid_of<CW>(P), CW::THREADS, P, e, stream)) != QWEN_OK) return rc;
     }
   }
   if (grad_hidden) {
-    int splits = b.splits;
+    int splits = b.splits, tiles_t = (tokens + CH::BT - 1) / CH::BT, tiles_n = (width + CH::BN - 1) / CH::BN;
     float unscale = 1.f / grad_scale<E>();
-    void* a[] = {&partial, &splits, &tokens, &width, &targets, &grad, &grad_stride, &unscale, &grad_hidden};
-    rc = launch((const void*)head_grad_hidden_kernel<T>, ((long)tokens * width / 8 + 255) / 256, 256, a, stream);
+    void* a[] = {&partial, &splits, &tiles_t, &tiles_n, &tokens, &width, &targets, &grad, &grad_stride, &unscale, &grad_hidden};
+    rc = launch((const void*)head_grad_hidden_kernel<CH>, (long)tiles_t * tiles_n * (CH::BN * CH::BT / 1024), 256, a, stream);
   }
   return rc;
 }
@@ -845,7 +922,7 @@ int product_i8(const signed char* a, const float* as, const signed char* b, cons
   e.ws = bs;
   e.tokens = tokens;
   e.rows = channels;
-  return launch_product(matmul_i8_kernel<C, T>, grid_of(P), C::THREADS, P, e, stream);
+  return launch_product(matmul_i8_kernel<C, T>, grid_of<C>(P), C::THREADS, P, e, stream);
 }
 }  // namespace
 
