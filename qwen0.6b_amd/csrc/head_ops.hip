@@ -12,6 +12,7 @@
 namespace hd {
 
 constexpr int CUS = 256;
+constexpr long CACHES = 32L << 20;  // the XCDs' L2 caches together
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 
 // targets as the caller holds them: 32- or 64-bit integers
@@ -59,7 +60,6 @@ __device__ __forceinline__ void join(float& m, float& s, float mo, float so) {
 // accumulators.
 template <class C>
 struct Stats : FromZero<C> {
-  static constexpr int STORES = 0;
   f32x2* part;  // [slot][tokens]
   float* tl;    // [tokens] target's logit
   Targets targets;
@@ -73,7 +73,7 @@ struct Stats : FromZero<C> {
       s[j] = 0.f;
     }
   }
-  __device__ __forceinline__ bool tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool last, int lane, int wn, int wt) {
+  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool last, int lane, int wn, int wt) {
     asm volatile("" : "+v"(lane));  // (as in Stores)
     const int n0 = at.tn * C::BN + 32 * C::NI * wn + 4 * (lane >> 5);  // register (i, q, r): row n0 + 32 i + 8 q + r
     const int t0 = at.tt * C::BT + 32 * C::NJ * wt + (lane & 31);
@@ -130,7 +130,6 @@ struct Stats : FromZero<C> {
       }
       reset();
     }
-    return false;
   }
 };
 
@@ -222,27 +221,27 @@ __global__ void __launch_bounds__(1024) head_total_kernel(const float* loss, Tar
 // each. make(i, q, j, v) turns the 4 accumulators of rows 32 i + 8 q + 4 (lane / 32) .. + 3 of the wave's (v, in
 // place) into what is stored; patch(ib, j) may then change numbers in LDS, and last(j, token, x) changes the
 // 16 bytes that go out for one of the wave's 32 tokens. Tokens from t_end and rows from n_end on are not stored.
-// Returns whether exactly COUNT stores were sent (not where some lanes' are left out).
+// STREAM: past the caches, for arrays that do not stay in them anyway (8-bit logits of 1919 positions, 583 MB,
+// 400 -> 348 us; the logits' gradient, which the next kernels read, is stored the ordinary way: 4% faster in all).
 // (The stores take a scalar base and a vector offset: with buffer stores that take a scalar offset of their own, now
 // and then 16 bytes of a tile were wrong.)
 struct Nothing {
   __device__ void operator()(int, int) const {}
   __device__ void operator()(int, int, u32x4&) const {}
 };
-template <class C, class T>
+template <class C, class T, bool STREAM>
 struct Stores {
   static constexpr int FIT = 4 / (int)sizeof(T);
   static constexpr int NB = C::NI < FIT ? C::NI : FIT;            // tiles of 32 rows staged at a time
   static constexpr int PER = 16 / sizeof(T), CH = 32 * NB / PER;  // numbers per 16 bytes, 16 bytes per token
   static_assert(C::NI % NB == 0 && NB >= 1, "a wave's staging area");
-  static constexpr int COUNT = C::NJ * (C::NI / NB) * (32 * CH / 64);
   typedef T t4 __attribute__((ext_vector_type(4)));
   typedef T tp __attribute__((ext_vector_type(PER)));
   // where the wave's LDS holds chunk c of token t
   static __device__ __forceinline__ u32 place(int t, int c) { return (u32)(t * CH * 16 + ((c ^ (t & (CH - 1))) << 4)); }
 
   template <class Make, class Patch, class Last>
-  static __device__ __forceinline__ bool store(typename C::E::acc (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wn,
+  static __device__ __forceinline__ void store(typename C::E::acc (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wn,
                                                int wt, char* lds, T* out, long ld, int t_end, int n_end, Make&& make,
                                                Patch&& patch, Last&& last) {
     // (what follows from `lane` is computed here, item by item, rather than kept in registers through the K loop)
@@ -281,7 +280,12 @@ struct Stores {
           u32x4 x = *(const u32x4*)(lds + place(t, cr));
           last(j, t, x);
           if (inner) {
-            *(u32x4*)(base + ((long)(32 * j + TP * p) * ld + 32 * ib) * (long)sizeof(T) + off) = x;
+            typedef __attribute__((address_space(1))) u32x4 global_u32x4;  // (made of integers, `base` could be in any memory)
+            global_u32x4* dst = (global_u32x4*)(base + ((long)(32 * j + TP * p) * ld + 32 * ib) * (long)sizeof(T) + off);
+            if (STREAM)
+              __builtin_nontemporal_store(x, dst);
+            else
+              *dst = x;
           } else if (t0 + 32 * j + t < t_end && n0 + 32 * ib + PER * cr < n_end) {
             const int n = n0 + 32 * ib + PER * cr;
             T* dst = out + (long)(t0 + 32 * j + t) * ld + n;
@@ -298,7 +302,6 @@ struct Stores {
         asm volatile("" ::: "memory");
       }
     }
-    return inner;
   }
 };
 
@@ -314,40 +317,44 @@ constexpr float grad_scale() { return sizeof(typename E::elem) == 2 && std::is_s
 template <class C>
 struct Softgrad : FromZero<C> {
   typedef typename C::E::elem T;
-  typedef Stores<C, T> St;
-  static constexpr int STORES = St::COUNT;
+  typedef Stores<C, T, false> St;
   T* out;  // [tokens_pad][ld]
   long ld;
   const float *loss, *lse;
   Targets targets;
   int tokens, tokens_pad, v0, rows, rows_pad;  // the piece: vocabulary rows v0 .. v0 + rows - 1
   char* lds;
-  __device__ __forceinline__ bool tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+  // what the lanes hold of their tokens, loaded when the token tile changes
+  int tile_t = -1;
+  float l2[C::NJ], own[C::NJ];
+  int row[C::NJ];     // the target's row of the piece, or out of it
+  u32 counts[C::NJ];  // a bit per token
+  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
     constexpr float SCALE = grad_scale<typename C::E>();
-    float l2[C::NJ], own[C::NJ];
-    int y[C::NJ];       // the target's row of the wave's, where it is one of them
-    u32 counts[C::NJ];  // a bit per token
+    if (at.tt != tile_t) {
+      tile_t = at.tt;
 #pragma unroll
-    for (int j = 0; j < C::NJ; ++j) {
-      const int t = at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31);
-      const long long target = t < tokens ? targets[t] : targets.ignore;
-      const bool c = t < tokens && target != targets.ignore;
-      counts[j] = (u32)__ballot(c);
-      const long long far = target - v0, row = far - (at.tn * C::BN + 32 * C::NI * wn);
-      y[j] = c && lane < 32 && far < rows && row >= 0 && row < 32 * C::NI ? (int)row : -1;
-      l2[j] = c ? fmaf(lse[t], LOG2E, -__builtin_log2f(SCALE)) : 0.f;
-      own[j] = c ? expm1f(-loss[t]) * SCALE : 0.f;  // the target's p - 1, also where p is nearly 1
+      for (int j = 0; j < C::NJ; ++j) {
+        const int t = at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31);
+        const long long target = t < tokens ? targets[t] : targets.ignore, far = target - v0;
+        const bool c = t < tokens && target != targets.ignore;
+        counts[j] = (u32)__ballot(c);
+        row[j] = c && lane < 32 && far >= 0 && far < rows ? (int)far : -1;
+        l2[j] = c ? fmaf(lse[t], LOG2E, -__builtin_log2f(SCALE)) : 0.f;
+        own[j] = c ? expm1f(-loss[t]) * SCALE : 0.f;  // the target's p - 1, also where p is nearly 1
+      }
     }
+    const int n0 = at.tn * C::BN + 32 * C::NI * wn;
     mask_rows<C>(acc, at, lane, wn, rows);
-    return St::store(
+    St::store(
         acc, at, lane, wn, wt, lds, out, ld, tokens_pad, rows_pad,
         [&](int, int, int j, float (&v)[4]) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = __builtin_amdgcn_exp2f(fmaf(v[r], LOG2E, -l2[j]));
         },
         [&](int ib, int j) {
-          const int n = y[j] - 32 * ib;
-          if (n >= 0 && n < 32 * St::NB) *(T*)(lds + St::place(lane & 31, n / St::PER) + (int)sizeof(T) * (n % St::PER)) = (T)own[j];
+          const int n = row[j] - n0 - 32 * ib;
+          if (row[j] >= 0 && n >= 0 && n < 32 * St::NB) *(T*)(lds + St::place(lane & 31, n / St::PER) + (int)sizeof(T) * (n % St::PER)) = (T)own[j];
         },
         [&](int j, int t, u32x4& x) {
           // (a mask: what a token that does not count holds may be NaN)
@@ -368,7 +375,6 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_softgrad_kernel(
 // per wave and store), carried on from one piece of the vocabulary to the next
 template <class C>
 struct Partials {
-  static constexpr int STORES = 0;
   float* out;  // [item][wave][i][j][q][lane][4]
   bool add;
   static __host__ __device__ __forceinline__ long place(long item, int wave, int i, int j) {
@@ -388,7 +394,7 @@ struct Partials {
           for (int r = 0; r < 4; ++r) acc[i][j][4 * q + r] = v[r];
         }
   }
-  __device__ __forceinline__ bool tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
     asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int i = 0; i < C::NI; ++i)
@@ -398,7 +404,6 @@ struct Partials {
         for (int q = 0; q < 4; ++q)
           *(f32x4*)(out + place(at.item, wt * C::WN + wn, i, j) + 256 * q + 4 * lane) =
               f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-    return false;
   }
 };
 template <class C>
@@ -472,14 +477,13 @@ __global__ void __launch_bounds__(256) head_weighted_rows_kernel(const T* hidden
 template <class C>
 struct WeightGrad : FromZero<C> {
   typedef typename C::E::elem T;
-  static constexpr int STORES = Stores<C, T>::COUNT;
   T* out;  // [rows][width]
   const float* top;
   int rows, width;
   char* lds;
-  __device__ __forceinline__ bool tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+  __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
     const float f = *top * (1.f / grad_scale<typename C::E>());
-    return Stores<C, T>::store(
+    Stores<C, T, true>::store(
         acc, at, lane, wn, wt, lds, out, width, rows, width,
         [&](int, int, int, float (&v)[4]) {
 #pragma unroll
@@ -498,18 +502,21 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_weight_grad_kern
 
 // ---- 8-bit integers --------------------------------------------------------------------
 
-template <class C, class T>
+template <class C, class T, bool STREAM>
 struct Dequant : FromZero<C> {
-  static constexpr int STORES = Stores<C, T>::COUNT;
   T* out;  // [tokens][rows]
   const float *xs, *ws;
   int tokens, rows;
   char* lds;
-  __device__ __forceinline__ bool tile(i32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+  int tile_t = -1;  // the token tile whose scales the lanes hold
+  float sx[C::NJ];
+  __device__ __forceinline__ void tile(i32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
     const int n0 = at.tn * C::BN + 32 * C::NI * wn + 4 * (lane >> 5);
-    float sx[C::NJ];
+    if (at.tt != tile_t) {
+      tile_t = at.tt;
 #pragma unroll
-    for (int j = 0; j < C::NJ; ++j) sx[j] = xs[min(at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31), tokens - 1)];
+      for (int j = 0; j < C::NJ; ++j) sx[j] = xs[min(at.tt * C::BT + 32 * (C::NJ * wt + j) + (lane & 31), tokens - 1)];
+    }
     // the rows' scales, 4 together (the wave's rows may end before its tile does)
     f32x4 sw[C::NI][4];
 #pragma unroll
@@ -524,7 +531,7 @@ struct Dequant : FromZero<C> {
           for (int r = 0; r < 4; ++r) sw[i][q][r] = ws[min(n + r, rows - 1)];
         }
       }
-    return Stores<C, T>::store(
+    Stores<C, T, STREAM>::store(
         acc, at, lane, wn, wt, lds, out, rows, tokens, rows,
         [&](int i, int q, int j, float (&v)[4]) {
 #pragma unroll
@@ -533,8 +540,8 @@ struct Dequant : FromZero<C> {
         Nothing(), Nothing());
   }
 };
-template <class C, class T>
-__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) matmul_i8_kernel(Product P, Dequant<C, T> epi) {
+template <class C, class T, bool STREAM>
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) matmul_i8_kernel(Product P, Dequant<C, T, STREAM> epi) {
   __shared__ __align__(16) char ring[C::RING];
   __shared__ __align__(16) char stage[C::STAGING];
   epi.lds = stage + (threadIdx.x >> 6) * 4096;
@@ -629,8 +636,49 @@ int launch_product(void (*kernel)(P, E), long grid, int threads, P product, E ep
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 long round_up(long x, long m) { return (x + m - 1) / m * m; }
 
+// The tiles a product can be cut into. Large ones do the most per byte that they bring to LDS, small ones leave no
+// CU idle where there are few, and two workgroups on a CU hide each other's waits (few tokens: the
+// head's rows then arrive as fast as memory gives them). SMALL is sized for the LDS that an epilogue leaves.
+enum TileKind : int { SMALL, MIDDLE, LARGE };
 template <class E, int LW = ROWS, int LX = ROWS>
-using Tile = Config<E, 256, 256, 2, 4, 2, 1, LW, LX>;
+struct Tiles {
+  typedef Config<E, 128, 64, 2, 2, 2, 2, LW, LX> Small;
+  typedef Config<E, 128, 128, 2, 2, 2, 2, LW, LX> Middle;
+  typedef Config<E, 256, 256, 2, 4, 2, 1, LW, LX> Large;
+};
+template <>
+struct Tiles<Int8, ROWS, ROWS> {
+  typedef Config<Int8, 64, 64, 2, 2, 3, 2> Small;
+  typedef Config<Int8, 128, 128, 2, 2, 2, 2> Middle;
+  typedef Config<Int8, 256, 256, 2, 4, 2, 1> Large;
+};
+template <class E>
+struct StatsTiles {  // (no stores through LDS: a deeper ring)
+  typedef Config<E, 128, 64, 2, 2, 3, 2> Small;
+  typedef Config<E, 128, 128, 2, 2, 2, 2> Middle;
+  typedef Config<E, 256, 256, 2, 4, 2, 1> Large;
+};
+
+// How long a product takes, in units of what a CU multiplies by large tiles: whole rounds of tiles over
+// the chip, each as long as its numbers at the rate that this tile reaches (measured on 1919 positions: 16-bit 1622, 921
+// and 562 us, 8-bit 909, 510 and 343).
+template <class C>
+long cost(int tokens, int rows, int splits, int percent) {
+  const long items = (long)splits * ((tokens + C::BT - 1) / C::BT) * ((rows + C::BN - 1) / C::BN);
+  const long rounds = (items + CUS * C::OCC - 1) / (CUS * C::OCC);
+  return rounds * C::OCC * C::BN * C::BT * 100 / percent;
+}
+template <class TS>
+TileKind pick(int tokens, int rows) {
+  const long s = cost<typename TS::Small>(tokens, rows, 1, 36), m = cost<typename TS::Middle>(tokens, rows, 1, 62),
+             l = cost<typename TS::Large>(tokens, rows, 1, 100);
+  return l <= m && l <= s ? LARGE : m <= s ? MIDDLE : SMALL;
+}
+// f(tile) for the tile of this kind
+template <class TS, class F>
+auto with_tile(TileKind k, F&& f) {
+  return k == SMALL ? f(typename TS::Small()) : k == MIDDLE ? f(typename TS::Middle()) : f(typename TS::Large());
+}
 
 // a product's tiles over [tokens][rows]
 template <class C>
@@ -737,22 +785,28 @@ int forward(const Head& h, float* loss, float* lse, float* total, char* ws, long
 struct BackwardPlan {
   int tokens_pad;   // K of grad_weight's product
   int rows;         // vocabulary rows per piece (a multiple of 256)
-  int splits, split_steps;  // of grad_hidden's product
+  TileKind kind;    // of grad_hidden's product (its partial sums are laid out by tile)
+  int splits, split_steps;
   long g, weighted, partial, top, bytes;  // places in the workspace
 };
-template <class E>
 BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
-  typedef Tile<E, COLS, ROWS> CH;
+  typedef Tiles<Half, COLS, ROWS> TS;
   BackwardPlan b;
   b.tokens_pad = (int)round_up(h.tokens, 64);
   // the gradient of the logits is kept for a piece of the vocabulary: 128 MB, half of the 256 MB cache before HBM
+  // (4096 positions: 64 MB 4380 us, 128 MB 3845, 256 MB 3977)
   constexpr long PIECE = 64L << 20;
   const long rows = PIECE / b.tokens_pad / 256 * 256, all = round_up(h.vocab, 256);
   b.rows = (int)(rows < 256 ? 256 : rows > all ? all : rows);
-  const long tiles = (long)((h.tokens + CH::BT - 1) / CH::BT) * ((h.width + CH::BN - 1) / CH::BN);
+  // of grad_hidden's sums over the vocabulary, as many parts as give every workgroup one
   const int steps = (int)(round_up(b.rows < h.vocab ? b.rows : h.vocab, 64) / 64);  // of the first piece; no other has more
-  long s = CUS / tiles;
-  b.splits = (int)(s < 1 ? 1 : s > steps ? steps : s);
+  b.kind = h.tokens <= 64 ? SMALL : h.tokens <= 128 ? MIDDLE : LARGE;
+  const long tile_numbers = with_tile<TS>(b.kind, [&](auto c) {
+    typedef decltype(c) C;
+    const long tiles = (long)((h.tokens + C::BT - 1) / C::BT) * ((h.width + C::BN - 1) / C::BN), s = CUS * C::OCC / tiles;
+    b.splits = (int)(s < 1 ? 1 : s > steps ? steps : s);
+    return tiles * C::BN * C::BT;
+  });
   b.split_steps = (steps + b.splits - 1) / b.splits;
   b.splits = (steps + b.split_steps - 1) / b.split_steps;
   long at = 0;
@@ -764,7 +818,7 @@ BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
   b.top = take(4);
   b.g = take(2L * b.tokens_pad * b.rows);
   b.weighted = take(want_weight ? 2L * b.tokens_pad * h.width : 0);
-  b.partial = take(want_hidden ? 4L * b.splits * tiles * CH::BN * CH::BT : 0);
+  b.partial = take(want_hidden ? 4L * b.splits * tile_numbers : 0);
   b.bytes = at;
   return b;
 }
@@ -773,10 +827,7 @@ template <class E>
 int backward(const Head& h, const float* grad, long grad_stride, const float* loss, const float* lse, void* grad_hidden,
              void* grad_weight, char* ws, long ws_bytes, hipStream_t stream) {
   typedef typename E::elem T;
-  typedef Tile<E> CG;
-  typedef Tile<E, COLS, ROWS> CH;
-  typedef Tile<E, COLS, COLS> CW;
-  const BackwardPlan b = backward_plan<E>(h, grad_hidden, grad_weight);
+  const BackwardPlan b = backward_plan(h, grad_hidden, grad_weight);
   if (ws_bytes < b.bytes) return QWEN_ERR_ARG;
   T* g = (T*)(ws + b.g);
   T* weighted = (T*)(ws + b.weighted);
@@ -797,10 +848,11 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* lo
   for (int v0 = 0; v0 < h.vocab; v0 += b.rows) {
     const int rows = h.vocab - v0 < b.rows ? h.vocab - v0 : b.rows, rows_pad = (int)round_up(rows, 64);
     const char* w = (const char*)h.weight + 2 * (long)v0 * h.weight_ld;
-    {
-      Product P = make_product<CG>(rows_of(h.hidden, h.hidden_ld, tokens, width), rows_of(w, h.weight_ld, rows, width),
-                                   k_steps(2L * width));
-      Softgrad<CG> e;
+    rc = with_tile<Tiles<E>>(pick<Tiles<E>>(tokens, rows), [&](auto c) {
+      typedef decltype(c) C;
+      Product P = make_product<C>(rows_of(h.hidden, h.hidden_ld, tokens, width), rows_of(w, h.weight_ld, rows, width),
+                                  k_steps(2L * width));
+      Softgrad<C> e;
       e.out = g;
       e.ld = b.rows;
       e.loss = loss;
@@ -811,38 +863,46 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* lo
       e.v0 = v0;
       e.rows = rows;
       e.rows_pad = rows_pad;
-      if ((rc = launch_product(head_softgrad_kernel<CG>, grid_of<CG>(P), CG::THREADS, P, e, stream)) != QWEN_OK) return rc;
-    }
+      return launch_product(head_softgrad_kernel<C>, grid_of<C>(P), C::THREADS, P, e, stream);
+    });
+    if (rc != QWEN_OK) return rc;
     if (grad_hidden) {
-      Operand x = {(const char*)g, 2L * b.rows, tokens, 2 * rows_pad};
-      Operand wt = {w, 2 * h.weight_ld, width, rows};
-      Product P = make_product<CH>(x, wt, rows_pad / 64);
-      P.split_steps = b.split_steps;
-      P.splits = (P.steps + P.split_steps - 1) / P.split_steps;
-      Partials<CH> e;
-      e.out = partial;
-      e.add = v0 > 0;
-      if ((rc = launch_product(head_partials_kernel<CH>, grid_of<CH>(P), CH::THREADS, P, e, stream)) != QWEN_OK) return rc;
+      rc = with_tile<Tiles<E, COLS, ROWS>>(b.kind, [&](auto c) {
+        typedef decltype(c) C;
+        Product P = make_product<C>(Operand{(const char*)g, 2L * b.rows, tokens, 2 * rows_pad},
+                                    Operand{w, 2 * h.weight_ld, width, rows}, rows_pad / 64);
+        P.split_steps = b.split_steps;
+        P.splits = (P.steps + P.split_steps - 1) / P.split_steps;
+        Partials<C> e;
+        e.out = partial;
+        e.add = v0 > 0;
+        return launch_product(head_partials_kernel<C>, grid_of<C>(P), C::THREADS, P, e, stream);
+      });
+      if (rc != QWEN_OK) return rc;
     }
     if (grad_weight) {
-      Operand x = {(const char*)g, 2L * b.rows, rows_pad, tokens_pad};
-      Operand wt = {(const char*)weighted, 2L * width, width, tokens_pad};
-      Product P = make_product<CW>(x, wt, tokens_pad / 64);
-      WeightGrad<CW> e;
-      e.out = (T*)grad_weight + (long)v0 * width;
-      e.top = top;
-      e.rows = rows;
-      e.width = width;
-      if ((rc = launch_product(head_weight_grad_kernel<CW>, grid_of<CW>(P), CW::THREADS, P, e, stream)) != QWEN_OK) return rc;
+      rc = with_tile<Tiles<E, COLS, COLS>>(tokens <= 128 ? MIDDLE : LARGE, [&](auto c) {
+        typedef decltype(c) C;
+        Product P = make_product<C>(Operand{(const char*)g, 2L * b.rows, rows_pad, tokens_pad},
+                                    Operand{(const char*)weighted, 2L * width, width, tokens_pad}, tokens_pad / 64);
+        WeightGrad<C> e;
+        e.out = (T*)grad_weight + (long)v0 * width;
+        e.top = top;
+        e.rows = rows;
+        e.width = width;
+        return launch_product(head_weight_grad_kernel<C>, grid_of<C>(P), C::THREADS, P, e, stream);
+      });
+      if (rc != QWEN_OK) return rc;
     }
   }
-  if (grad_hidden) {
-    int splits = b.splits, tiles_t = (tokens + CH::BT - 1) / CH::BT, tiles_n = (width + CH::BN - 1) / CH::BN;
+  if (!grad_hidden) return rc;
+  return with_tile<Tiles<E, COLS, ROWS>>(b.kind, [&](auto c) {
+    typedef decltype(c) C;
+    int splits = b.splits, tiles_t = (tokens + C::BT - 1) / C::BT, tiles_n = (width + C::BN - 1) / C::BN;
     float unscale = 1.f / grad_scale<E>();
     void* a[] = {&partial, &splits, &tiles_t, &tiles_n, &tokens, &width, &targets, &grad, &grad_stride, &unscale, &grad_hidden};
-    rc = launch((const void*)head_grad_hidden_kernel<CH>, (long)tiles_t * tiles_n * (CH::BN * CH::BT / 1024), 256, a, stream);
-  }
-  return rc;
+    return launch((const void*)head_grad_hidden_kernel<C>, (long)tiles_t * tiles_n * (C::BN * C::BT / 1024), 256, a, stream);
+  });
 }
 
 }  // namespace
@@ -853,7 +913,7 @@ using namespace hd;
 extern "C" long long qwen_cross_entropy_workspace(int tokens, int vocab, int width) {
   if (tokens < 1 || tokens > MAX_TOKENS || vocab < 1 || vocab > MAX_VOCAB || width < 8) return 0;
   Head h = {nullptr, 0, nullptr, 0, {}, tokens, vocab, width};
-  return forward_bytes<Tile<Half>>(h);
+  return with_tile<StatsTiles<Half>>(pick<StatsTiles<Half>>(tokens, vocab), [&](auto c) { return forward_bytes<decltype(c)>(h); });
 }
 
 extern "C" int qwen_cross_entropy(const void* hidden, long long hidden_stride, const void* weight, long long weight_stride,
@@ -867,14 +927,15 @@ extern "C" int qwen_cross_entropy(const void* hidden, long long hidden_stride, c
   if (tokens == 0) return QWEN_OK;
   if (!loss || !lse || !workspace || !aligned16(workspace)) return QWEN_ERR_ARG;
   char* ws = (char*)workspace;
-  return dtype == QWEN_F16 ? forward<Tile<Half>>(h, loss, lse, total, ws, workspace_bytes, stream)
-                           : forward<Tile<Bfloat>>(h, loss, lse, total, ws, workspace_bytes, stream);
+  const TileKind k = pick<StatsTiles<Half>>(tokens, vocab);
+  auto run = [&](auto c) { return forward<decltype(c)>(h, loss, lse, total, ws, workspace_bytes, stream); };
+  return dtype == QWEN_F16 ? with_tile<StatsTiles<Half>>(k, run) : with_tile<StatsTiles<Bfloat>>(k, run);
 }
 
 extern "C" long long qwen_cross_entropy_backward_workspace(int tokens, int vocab, int width, int want_hidden, int want_weight) {
   if (tokens < 1 || tokens > MAX_TOKENS || vocab < 1 || vocab > MAX_VOCAB || width < 8) return 0;
   Head h = {nullptr, 0, nullptr, 0, {}, tokens, vocab, width};
-  return backward_plan<Half>(h, want_hidden != 0, want_weight != 0).bytes;
+  return backward_plan(h, want_hidden != 0, want_weight != 0).bytes;
 }
 
 extern "C" int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const void* hidden,
@@ -910,19 +971,29 @@ extern "C" int qwen_quantize_rows(const void* x, long long stride, int rows, int
 
 namespace hd {
 namespace {
-template <class T>
+template <class C, class T, bool STREAM>
 int product_i8(const signed char* a, const float* as, const signed char* b, const float* bs, void* out, int tokens,
                int channels, int width, hipStream_t stream) {
-  typedef Tile<Int8> C;
   Product P = make_product<C>(Operand{(const char*)a, width, tokens, width}, Operand{(const char*)b, width, channels, width},
                               k_steps(width));
-  Dequant<C, T> e;
+  Dequant<C, T, STREAM> e;
   e.out = (T*)out;
   e.xs = as;
   e.ws = bs;
   e.tokens = tokens;
   e.rows = channels;
-  return launch_product(matmul_i8_kernel<C, T>, grid_of<C>(P), C::THREADS, P, e, stream);
+  return launch_product(matmul_i8_kernel<C, T, STREAM>, grid_of<C>(P), C::THREADS, P, e, stream);
+}
+template <class T>
+int product_i8(const signed char* a, const float* as, const signed char* b, const float* bs, void* out, int tokens,
+               int channels, int width, hipStream_t stream) {
+  typedef Tiles<Int8> TS;
+  return with_tile<TS>(pick<TS>(tokens, channels), [&](auto c) {
+    typedef decltype(c) C;
+    if ((long)tokens * channels * (long)sizeof(T) > CACHES)
+      return product_i8<C, T, true>(a, as, b, bs, out, tokens, channels, width, stream);
+    return product_i8<C, T, false>(a, as, b, bs, out, tokens, channels, width, stream);
+  });
 }
 }  // namespace
 
