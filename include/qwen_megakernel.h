@@ -175,6 +175,16 @@ int qwen_prefill(
     int num_layers, int start_position, int max_seq_len, float attn_scale,
     hipStream_t stream);
 
+/* qwen_prefill that also gives what the lm_head takes at every one of its positions: hidden_rows
+ * (fp16 [n][1024], 16-byte aligned) receives the final-layer residual's RMSNorm times
+ * final_norm_weight (fp16 [1024]), rounded once. Everything else as qwen_prefill. */
+int qwen_prefill_hidden(
+    const int* ids, int n, const void* embed_weight,
+    const LDGLayerWeight* layer_weights, const void* final_norm_weight,
+    const void* cos_table, const void* sin_table, void* k_cache, void* v_cache,
+    void* hidden_buffer, void* hidden_rows, int num_layers, int start_position,
+    int max_seq_len, float attn_scale, hipStream_t stream);
+
 /* Profiling aid for qwen_prefill: the wall-clock times (s_memrealtime ticks,
  * 100 MHz) at which the last prefill on the current device started and passed
  * each of its grid barriers: [0] start, [1] after the embedding, then for each
@@ -257,8 +267,8 @@ int qwen_mlp_block(const void* x_f16, const void* post_norm_weight, const void* 
  * w_v of `weight` ([vocab][weight_stride], the same dtype)
  *   lse[t]  = log sum_v exp(h_t . w_v)                (fp32 [tokens])
  *   loss[t] = lse[t] - h_t . w_target                 (fp32 [tokens])
- * and, with `total` (nullable, fp32 [2]), the sum of the losses and the number of positions that
- * count. targets: device integers of target_bits (32 or 64) bits; a target equal to ignore_index does
+ * and, with `total` (nullable, fp32 [3]), the sum of the losses, the number of positions that count and
+ * the mean. targets: device integers of target_bits (32 or 64) bits; a target equal to ignore_index does
  * not count (loss 0), one outside [0, vocab) otherwise gives a NaN loss. Sums are fp32, in an order
  * that depends on the sizes only: the same call always gives the same bits.
  * width: a multiple of 8; the strides (in elements): multiples of 8, at least width and at most
@@ -272,16 +282,17 @@ int qwen_cross_entropy(const void* hidden, long long hidden_stride, const void* 
                        long long workspace_bytes, hipStream_t stream);
 
 /* Its gradients: with p_tv = exp(h_t . w_v - lse[t]) and g_t = grad_loss[t * grad_stride] (fp32; stride
- * 0: one number for all positions)
+ * 0: one number for all positions), over *grad_divisor where that is not null (a mean's total[1])
  *   grad_hidden[t] = g_t sum_v (p_tv - [v = target_t]) w_v     ([tokens][width])
  *   grad_weight[v] = sum_t g_t (p_tv - [v = target_t]) h_t     ([vocab][width])
  * in the inputs' dtype; either may be null. loss and lse are what qwen_cross_entropy gave for the same inputs.
- * Positions that do not count take no part (their hidden rows may hold anything) and get a zero row.
+ * Positions that do not count take no part (their hidden rows may hold anything) and get a zero row; those with a
+ * NaN loss give NaN.
  * The logits are computed again, a piece of the vocabulary at a time; p - [v = target] is rounded to the inputs' dtype
  * for the matrix cores, sums are fp32, one rounding at the end. Same limits; tokens >= 1. */
 long long qwen_cross_entropy_backward_workspace(int tokens, int vocab, int width, int want_hidden, int want_weight);
-int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const void* hidden,
-                                long long hidden_stride, const void* weight, long long weight_stride,
+int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const float* grad_divisor,
+                                const void* hidden, long long hidden_stride, const void* weight, long long weight_stride,
                                 const void* targets, int target_bits, int tokens, int vocab, int width, int dtype,
                                 long long ignore_index, const float* loss, const float* lse, void* grad_hidden,
                                 void* grad_weight, void* workspace, long long workspace_bytes, hipStream_t stream);
@@ -295,8 +306,8 @@ int qwen_quantize_rows(const void* x, long long stride, int rows, int width, int
 
 /* Matrix product in 8-bit integers: out[t][n] = a_scale[t] b_scale[n] sum_k a[t][k] b[n][k], with
  * a int8 [tokens][width], b int8 [channels][width], out [tokens][channels] in out_dtype (QWEN_F16,
- * QWEN_BF16 or QWEN_F32). The sum is exact; the scaling is fp32, rounded once to out_dtype. width: a multiple of 16,
- * at most 65536; a, b and out 16-byte aligned. */
+ * QWEN_BF16 or QWEN_F32). The sum is exact; the scaling is fp32, rounded once to out_dtype. width: a multiple
+ * of 16, at most 65536; channels: at most 4194304; a, b and out 16-byte aligned. */
 int qwen_matmul_i8(const signed char* a, const float* a_scale, const signed char* b, const float* b_scale, void* out,
                    int out_dtype, int tokens, int channels, int width, hipStream_t stream);
 

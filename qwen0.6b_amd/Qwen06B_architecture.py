@@ -13,6 +13,8 @@ Differences from the reference, all additive:
 * ``load_weights`` reads a local Hugging Face checkpoint directory
   (safetensors) instead of downloading; ``qwen_weights.synthetic_weights``
   builds seeded random weights in the same dictionary layout;
+* ``Decoder.hidden_states`` / ``score`` / ``quantize_head`` / ``logits`` and ``lm_head_loss`` work on every position
+  of a text: its log-probability, its logits from an 8-bit head, a loss with gradients;
 * ``Decoder.prefill`` / ``generate_ids`` run a prompt and greedy generation on
   token ids (no tokenizer needed); the prompt is prefilled in one launch of the
   batched (MFMA) prefill kernel instead of one launch and host sync per token;
@@ -224,41 +226,25 @@ def _pack_layer_weights(layer_weights: list) -> torch.Tensor:
 
 
 class _HeadLoss(torch.autograd.Function):
-    """Cross entropy of every position against the head, and [sum, count] of the positions that count."""
+    """Cross entropy against the head: of every position, or their sum, or their mean."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index):
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
         loss, lse, total = qwen_megakernel_C.lm_head_cross_entropy_total(hidden, weight, targets, ignore_index)
-        ctx.save_for_backward(hidden, weight, targets, loss, lse)
+        # (total.data: a caller's in-place change of the scalar is not one of the count)
+        ctx.save_for_backward(hidden, weight, targets, loss, lse, total.data)
         ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(total)
-        return loss, total
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_loss, _):
-        hidden, weight, targets, loss, lse = ctx.saved_tensors
-        grads = qwen_megakernel_C.lm_head_cross_entropy_backward(
-            grad_loss, hidden, weight, targets, loss, lse, ctx.ignore_index, *ctx.needs_input_grad[:2])
-        return (*grads, None, None)
-
-
-class _MeanOfLosses(torch.autograd.Function):
-    """The losses' sum, or their mean over the positions that count, from the total that came with them."""
-
-    @staticmethod
-    def forward(ctx, loss, total, mean):
-        ctx.positions = loss.shape[0]
-        ctx.mean = mean
-        ctx.save_for_backward(total)
-        return total[0] / total[1] if mean else total[0].clone()
+        ctx.reduction = reduction
+        return loss if reduction == "none" else total[0 if reduction == "sum" else 2]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        (total,) = ctx.saved_tensors
-        grad = grad / total[1] if ctx.mean else grad
-        return grad.expand(ctx.positions), None, None
+        hidden, weight, targets, loss, lse, total = ctx.saved_tensors
+        grads = qwen_megakernel_C.lm_head_cross_entropy_backward(
+            grad if ctx.reduction == "none" else grad.expand(loss.shape), hidden, weight, targets, loss, lse,
+            ctx.ignore_index, *ctx.needs_input_grad[:2], total[1] if ctx.reduction == "mean" else None)
+        return (*grads, None, None, None)
 
 
 def lm_head_loss(hidden, weight, targets, ignore_index: int = -100, reduction: str = "mean"):
@@ -269,8 +255,7 @@ def lm_head_loss(hidden, weight, targets, ignore_index: int = -100, reduction: s
     in any fp16 training."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
-    loss, total = _HeadLoss.apply(hidden, weight, targets, ignore_index)
-    return loss if reduction == "none" else _MeanOfLosses.apply(loss, total, reduction == "mean")
+    return _HeadLoss.apply(hidden, weight, targets, ignore_index, reduction)
 
 
 class Decoder:
@@ -401,6 +386,53 @@ class Decoder:
         last = int(out[-1].item())
         _check_device_errors()
         return last
+
+    def hidden_states(self, ids) -> torch.Tensor:
+        """Prefill ``ids`` at the next positions; returns the final-normed hidden row of each, fp16
+        [len(ids), 1024] on the device: what the lm_head takes, for ``lm_head_loss`` and ``logits``."""
+        ids = [int(t) for t in ids]
+        if not ids:
+            raise ValueError("hidden_states needs at least one id")
+        if self._position + len(ids) > MAX_SEQ_LEN:
+            raise RuntimeError(f"prefill of {len(ids)} ids at position {self._position} exceeds {MAX_SEQ_LEN}")
+        t = torch.from_numpy(np.asarray(ids, dtype=np.int32)).to(DEVICE)
+        rows = _require_megakernel_op("prefill_hidden")(
+            t, self._embed_weight, self._layer_weights_packed, self._final_norm_weight, self._cos_table,
+            self._sin_table, self._k_cache, self._v_cache, self._hidden, self._num_layers, self._position,
+            MAX_SEQ_LEN, self._attn_scale)
+        self._position += len(ids)
+        return rows
+
+    def score(self, ids) -> torch.Tensor:
+        """Log-probability of each id after the first given those before it, fp32 [len(ids) - 1] on the
+        device (perplexity: ``exp(-score(ids).mean())``): one prefill of ids[:-1] from position 0 and one
+        cross entropy against the lm_head, without logits in memory."""
+        ids = [int(t) for t in ids]
+        if len(ids) < 2:
+            raise ValueError("score needs at least two ids")
+        if any(not 0 <= t < VOCAB_SIZE for t in ids):
+            raise ValueError(f"ids outside [0, {VOCAB_SIZE})")
+        self.reset()
+        rows = self.hidden_states(ids[:-1])
+        targets = torch.from_numpy(np.asarray(ids[1:], dtype=np.int32)).to(DEVICE)
+        loss, _ = _require_megakernel_op("lm_head_cross_entropy")(rows, self._lm_head_weight, targets)
+        _check_device_errors()
+        return -loss
+
+    def quantize_head(self):
+        """The lm_head's rows in 8-bit integers with a scale each, (int8 [151936, 1024], fp32 [151936]):
+        half the memory traffic, for ``logits``. The caller keeps them."""
+        return _require_megakernel_op("quantize_rows")(self._lm_head_weight)
+
+    def logits(self, ids, head8, out_dtype=torch.float32) -> torch.Tensor:
+        """Prefill ``ids`` at the next positions; returns the logits of every one of them, [len(ids), 151936],
+        from the 8-bit head ``head8`` (see ``quantize_head``): hidden rows rounded to 8 bits with a scale per
+        position, products and sums exact in integers."""
+        rows = self.hidden_states(ids)
+        q, scale = _require_megakernel_op("quantize_rows")(rows)
+        out = _require_megakernel_op("matmul_i8")(q, scale, *head8, out_dtype)
+        _check_device_errors()
+        return out
 
     def generate_until(self, first_token_id: int, max_tokens: int, eos_token_id: int) -> list:
         """Up to ``max_tokens`` greedy steps in one launch that end on the device after the

@@ -25,6 +25,19 @@ struct Targets {
   }
 };
 
+// the upstream gradient of each position: g[t stride], over *divisor where there is one
+struct Upstream {
+  const float* g;
+  long stride;
+  const float* divisor;
+  __device__ __forceinline__ float operator[](int t) const {
+    const float x = g[t * stride];
+    if (!divisor) return x;
+    const float d = *divisor;
+    return d == 0.f ? 0.f : x / d;  // (a mean of no positions: none has a gradient)
+  }
+};
+
 // ---- forward: running softmax statistics over the vocabulary ---------------------------
 
 // First workgroup whose share of `items` holds item x, of `grid` (run_product's deal)
@@ -185,7 +198,7 @@ __global__ void __launch_bounds__(JT* JS) head_join_kernel(const f32x2* part, co
   }
 }
 
-// sum of the losses and number of the positions that count, in a fixed order
+// sum of the losses (in a fixed order), number of the positions that count, mean
 __global__ void __launch_bounds__(1024) head_total_kernel(const float* loss, Targets targets, int tokens, float* total) {
   __shared__ float sm[16];
   __shared__ int cn[16];
@@ -212,6 +225,7 @@ __global__ void __launch_bounds__(1024) head_total_kernel(const float* loss, Tar
   }
   total[0] = s;
   total[1] = (float)n;
+  total[2] = s / (float)n;
 }
 
 // ---- stores of a tile ------------------------------------------------------------------
@@ -340,8 +354,10 @@ struct Softgrad : FromZero<C> {
         const bool c = t < tokens && target != targets.ignore;
         counts[j] = (u32)__ballot(c);
         row[j] = c && lane < 32 && far >= 0 && far < rows ? (int)far : -1;
-        l2[j] = c ? fmaf(lse[t], LOG2E, -__builtin_log2f(SCALE)) : 0.f;
-        own[j] = c ? expm1f(-loss[t]) * SCALE : 0.f;  // the target's p - 1, also where p is nearly 1
+        const float x = c ? loss[t] : 0.f;
+        // (a NaN loss: a target that is no row of the head, or logits that are NaN)
+        l2[j] = c ? (x == x ? fmaf(lse[t], LOG2E, -__builtin_log2f(SCALE)) : NAN) : 0.f;
+        own[j] = expm1f(-x) * SCALE;  // the target's p - 1, also where p is nearly 1
       }
     }
     const int n0 = at.tn * C::BN + 32 * C::NI * wn;
@@ -415,8 +431,8 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_partials_kernel(
 // grad_hidden: the splits' sums in order, times the position's upstream gradient; a thread has 4 numbers of one row
 template <class C>
 __global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part, int splits, int tiles_t, int tiles_n,
-                                                               int tokens, int width, Targets targets, const float* grad,
-                                                               long grad_stride, float unscale, typename C::E::elem* out) {
+                                                               int tokens, int width, Targets targets, Upstream grad,
+                                                               float unscale, typename C::E::elem* out) {
   typedef typename C::E::elem T;
   constexpr int PER_TILE = C::BN * C::BT / 4;
   const long e = (long)blockIdx.x * 256 + threadIdx.x;
@@ -428,19 +444,18 @@ __global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
   if (targets[t] != targets.ignore) {
     for (int s = 0; s < splits; ++s) a += *(const f32x4*)(part + ((long)s * tiles_t * tiles_n * PER_TILE + e) * 4);
-    a *= grad[t * grad_stride] * unscale;
+    a *= grad[t] * unscale;
   }
   typedef T t4 __attribute__((ext_vector_type(4)));
   *(t4*)(out + (long)t * width + n) = t4{(T)a[0], (T)a[1], (T)a[2], (T)a[3]};
 }
 
 // max |upstream gradient| of the positions that count
-__global__ void __launch_bounds__(1024) head_grad_max_kernel(const float* grad, long stride, Targets targets, int tokens,
-                                                             float* out) {
+__global__ void __launch_bounds__(1024) head_grad_max_kernel(Upstream grad, Targets targets, int tokens, float* out) {
   __shared__ float sm[16];
   float m = 0.f;
   for (int t = threadIdx.x; t < tokens; t += 1024)
-    if (targets[t] != targets.ignore) m = fmaxf(m, fabsf(grad[t * stride]));
+    if (targets[t] != targets.ignore) m = fmaxf(m, fabsf(grad[t]));
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
@@ -451,12 +466,12 @@ __global__ void __launch_bounds__(1024) head_grad_max_kernel(const float* grad, 
 }
 
 // The hidden rows as grad_weight's product takes them: each times its upstream gradient over the largest one
-// (1, and no rounding, where all positions weigh the same), zeros for positions that do not count and
-// up to a whole number of K steps
+// (1 or -1, and no rounding, where all positions weigh the same), zeros for positions that do not count
+// and up to a whole number of K steps. top: the largest, or null where there is only one.
 template <class T>
-__global__ void __launch_bounds__(256) head_weighted_rows_kernel(const T* hidden, long ld, Targets targets, const float* grad,
-                                                                 long grad_stride, const float* top, int tokens,
-                                                                 int tokens_pad, int width, T* out) {
+__global__ void __launch_bounds__(256) head_weighted_rows_kernel(const T* hidden, long ld, Targets targets, Upstream grad,
+                                                                 const float* top, int tokens, int tokens_pad, int width,
+                                                                 T* out) {
   const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
   if (e >= (long)tokens_pad * width) return;
   const int t = (int)(e / width), c = (int)(e % width);
@@ -465,7 +480,7 @@ __global__ void __launch_bounds__(256) head_weighted_rows_kernel(const T* hidden
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = (T)0.f;
   if (t < tokens && targets[t] != targets.ignore) {
-    const float m = *top, g = m == 0.f ? 0.f : grad[t * grad_stride] / m;
+    const float m = top ? *top : fabsf(grad[0]), g = m == 0.f ? 0.f : grad[t] / m;
     const t8 h = *(const t8*)(hidden + t * ld + c);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = (T)((float)h[k] * g);
@@ -478,11 +493,12 @@ template <class C>
 struct WeightGrad : FromZero<C> {
   typedef typename C::E::elem T;
   T* out;  // [rows][width]
-  const float* top;
+  Upstream grad;
+  const float* top;  // as in head_weighted_rows_kernel
   int rows, width;
   char* lds;
   __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
-    const float f = *top * (1.f / grad_scale<typename C::E>());
+    const float f = (top ? *top : fabsf(grad[0])) * (1.f / grad_scale<typename C::E>());
     Stores<C, T, true>::store(
         acc, at, lane, wn, wt, lds, out, width, rows, width,
         [&](int, int, int, float (&v)[4]) {
@@ -710,7 +726,7 @@ struct Head {
 };
 
 constexpr long MAX_ROW_BYTES = 4L << 20;  // a tile's offsets stay below 2^31
-constexpr int MAX_TOKENS = 1 << 20, MAX_VOCAB = 1 << 24;
+constexpr int MAX_TOKENS = 1 << 20, MAX_VOCAB = 1 << 24, MAX_CHANNELS = 1 << 22;
 
 int check_head(const Head& h, int target_bits, int dtype) {
   if (h.tokens < 0 || h.tokens > MAX_TOKENS || h.vocab < 1 || h.vocab > MAX_VOCAB || h.width < 8 || h.width % 8 != 0)
@@ -824,7 +840,7 @@ BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
 }
 
 template <class E>
-int backward(const Head& h, const float* grad, long grad_stride, const float* loss, const float* lse, void* grad_hidden,
+int backward(const Head& h, Upstream grad, const float* loss, const float* lse, void* grad_hidden,
              void* grad_weight, char* ws, long ws_bytes, hipStream_t stream) {
   typedef typename E::elem T;
   const BackwardPlan b = backward_plan(h, grad_hidden, grad_weight);
@@ -837,11 +853,15 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* lo
   int tokens = h.tokens, tokens_pad = b.tokens_pad, width = h.width;
   int rc = QWEN_OK;
   if (grad_weight) {
-    void* a[] = {&grad, &grad_stride, &targets, &tokens, &top};
-    if ((rc = launch((const void*)head_grad_max_kernel, 1, 1024, a, stream)) != QWEN_OK) return rc;
+    if (grad.stride == 0) {
+      top = nullptr;  // one number for all positions
+    } else {
+      void* a[] = {&grad, &targets, &tokens, &top};
+      if ((rc = launch((const void*)head_grad_max_kernel, 1, 1024, a, stream)) != QWEN_OK) return rc;
+    }
     const T* hidden = (const T*)h.hidden;
     long ld = h.hidden_ld;
-    void* c[] = {&hidden, &ld, &targets, &grad, &grad_stride, &top, &tokens, &tokens_pad, &width, &weighted};
+    void* c[] = {&hidden, &ld, &targets, &grad, &top, &tokens, &tokens_pad, &width, &weighted};
     rc = launch((const void*)head_weighted_rows_kernel<T>, ((long)tokens_pad * width / 8 + 255) / 256, 256, c, stream);
     if (rc != QWEN_OK) return rc;
   }
@@ -887,6 +907,7 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* lo
                                     Operand{(const char*)weighted, 2L * width, width, tokens_pad}, tokens_pad / 64);
         WeightGrad<C> e;
         e.out = (T*)grad_weight + (long)v0 * width;
+        e.grad = grad;
         e.top = top;
         e.rows = rows;
         e.width = width;
@@ -900,7 +921,7 @@ int backward(const Head& h, const float* grad, long grad_stride, const float* lo
     typedef decltype(c) C;
     int splits = b.splits, tiles_t = (tokens + C::BT - 1) / C::BT, tiles_n = (width + C::BN - 1) / C::BN;
     float unscale = 1.f / grad_scale<E>();
-    void* a[] = {&partial, &splits, &tiles_t, &tiles_n, &tokens, &width, &targets, &grad, &grad_stride, &unscale, &grad_hidden};
+    void* a[] = {&partial, &splits, &tiles_t, &tiles_n, &tokens, &width, &targets, &grad, &unscale, &grad_hidden};
     return launch((const void*)head_grad_hidden_kernel<C>, (long)tiles_t * tiles_n * (C::BN * C::BT / 1024), 256, a, stream);
   });
 }
@@ -938,8 +959,8 @@ extern "C" long long qwen_cross_entropy_backward_workspace(int tokens, int vocab
   return backward_plan(h, want_hidden != 0, want_weight != 0).bytes;
 }
 
-extern "C" int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const void* hidden,
-                                           long long hidden_stride, const void* weight, long long weight_stride,
+extern "C" int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const float* grad_divisor,
+                                           const void* hidden, long long hidden_stride, const void* weight, long long weight_stride,
                                            const void* targets, int target_bits, int tokens, int vocab, int width,
                                            int dtype, long long ignore_index, const float* loss, const float* lse,
                                            void* grad_hidden, void* grad_weight, void* workspace,
@@ -952,9 +973,9 @@ extern "C" int qwen_cross_entropy_backward(const float* grad_loss, long long gra
       !aligned16(grad_weight) || !workspace || !aligned16(workspace))
     return QWEN_ERR_ARG;
   char* ws = (char*)workspace;
-  return dtype == QWEN_F16
-             ? backward<Half>(h, grad_loss, (long)grad_stride, loss, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream)
-             : backward<Bfloat>(h, grad_loss, (long)grad_stride, loss, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream);
+  const Upstream grad = {grad_loss, (long)grad_stride, grad_divisor};
+  return dtype == QWEN_F16 ? backward<Half>(h, grad, loss, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream)
+                           : backward<Bfloat>(h, grad, loss, lse, grad_hidden, grad_weight, ws, workspace_bytes, stream);
 }
 
 extern "C" int qwen_quantize_rows(const void* x, long long stride, int rows, int width, int dtype, signed char* q,
@@ -1009,7 +1030,7 @@ int norm_rows(const float* x, const void* gain, int rows, void* out, hipStream_t
 extern "C" int qwen_matmul_i8(const signed char* a, const float* a_scale, const signed char* b, const float* b_scale,
                               void* out, int out_dtype, int tokens, int channels, int width, hipStream_t stream) {
   // 65536 products of 8-bit numbers stay within 2^30
-  if (tokens < 0 || channels < 0 || width < 16 || width % 16 != 0 || width > 65536) return QWEN_ERR_ARG;
+  if (tokens < 0 || channels < 0 || channels > MAX_CHANNELS || width < 16 || width % 16 != 0 || width > 65536) return QWEN_ERR_ARG;
   if (out_dtype != QWEN_F16 && out_dtype != QWEN_BF16 && out_dtype != QWEN_F32) return QWEN_ERR_ARG;
   if (tokens == 0 || channels == 0) return QWEN_OK;
   if (!a || !a_scale || !b || !b_scale || !out || !aligned16(a) || !aligned16(b) || !aligned16(out)) return QWEN_ERR_ARG;

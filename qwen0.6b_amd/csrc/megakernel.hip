@@ -51,6 +51,10 @@
 
 using namespace ql;
 
+namespace hd {  // head_ops.hip
+int norm_rows(const float* x, const void* gain, int rows, void* out, hipStream_t stream);
+}
+
 typedef unsigned int u32;
 typedef unsigned long long u64;
 typedef u32 v4u __attribute__((ext_vector_type(4)));
@@ -750,10 +754,12 @@ extern "C" int qwen_generate_nosync_noalloc(int first_token_id, int num_steps, c
   return launch(P, stream, /*fixed=*/true);
 }
 
-extern "C" int qwen_prefill(const int* ids, int n, const void* embed_weight, const LDGLayerWeight* layer_weights,
-                            const void* cos_table, const void* sin_table, void* k_cache, void* v_cache,
-                            void* hidden_buffer, int num_layers, int start_position, int max_seq_len,
-                            float attn_scale, hipStream_t stream) {
+namespace {
+
+// qwen_prefill, and with hidden_rows the final norm of every position's residual into it
+int prefill(const int* ids, int n, const void* embed_weight, const LDGLayerWeight* layer_weights, const void* final_norm,
+            const void* cos_table, const void* sin_table, void* k_cache, void* v_cache, void* hidden_buffer,
+            void* hidden_rows, int num_layers, int start_position, int max_seq_len, float attn_scale, hipStream_t stream) {
   if (!ids || !embed_weight || !layer_weights || !cos_table || !sin_table || !k_cache || !v_cache || !hidden_buffer)
     return QWEN_ERR_ARG;
   if (!aligned16(embed_weight) || !aligned16(layer_weights) || !aligned16(cos_table) || !aligned16(sin_table) ||
@@ -809,7 +815,30 @@ extern "C" int qwen_prefill(const int* ids, int n, const void* embed_weight, con
   if ((rc = capture_state(stream, &captured)) != QWEN_OK || (rc = order_after(st, stream, captured)) != QWEN_OK) return rc;
   if (zero_words(P.bar, PF_BAR_BYTES, stream) != QWEN_OK) return QWEN_ERR_LAUNCH;
   void* args[] = {&P};
-  return launch_resident(st, PREFILL + cls, args, stream, captured);
+  if ((rc = launch_resident(st, PREFILL + cls, args, stream, captured)) != QWEN_OK || !hidden_rows) return rc;
+  // the workspace is the next call's only when its residual rows have been read
+  if ((rc = hd::norm_rows(P.X, final_norm, n, hidden_rows, stream)) != QWEN_OK) return rc;
+  if (captured) return capture_event(stream, st->order, /*record=*/true);
+  return hipEventRecord(st->order, stream) == hipSuccess ? QWEN_OK : QWEN_ERR_LAUNCH;
+}
+
+}  // namespace
+
+extern "C" int qwen_prefill(const int* ids, int n, const void* embed_weight, const LDGLayerWeight* layer_weights,
+                            const void* cos_table, const void* sin_table, void* k_cache, void* v_cache,
+                            void* hidden_buffer, int num_layers, int start_position, int max_seq_len,
+                            float attn_scale, hipStream_t stream) {
+  return prefill(ids, n, embed_weight, layer_weights, nullptr, cos_table, sin_table, k_cache, v_cache, hidden_buffer,
+                 nullptr, num_layers, start_position, max_seq_len, attn_scale, stream);
+}
+
+extern "C" int qwen_prefill_hidden(const int* ids, int n, const void* embed_weight, const LDGLayerWeight* layer_weights,
+                                   const void* final_norm_weight, const void* cos_table, const void* sin_table,
+                                   void* k_cache, void* v_cache, void* hidden_buffer, void* hidden_rows, int num_layers,
+                                   int start_position, int max_seq_len, float attn_scale, hipStream_t stream) {
+  if (!final_norm_weight || !hidden_rows || !aligned16(final_norm_weight) || !aligned16(hidden_rows)) return QWEN_ERR_ARG;
+  return prefill(ids, n, embed_weight, layer_weights, final_norm_weight, cos_table, sin_table, k_cache, v_cache,
+                 hidden_buffer, hidden_rows, num_layers, start_position, max_seq_len, attn_scale, stream);
 }
 
 extern "C" int qwen_prefill_timestamps(unsigned long long* out, int max_entries) {

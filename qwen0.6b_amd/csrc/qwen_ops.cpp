@@ -11,6 +11,7 @@
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cmath>
 #include <cstdint>
 #include <string>
 #include <tuple>
@@ -230,9 +231,10 @@ std::tuple<torch::Tensor, torch::Tensor> generate_sampled(
 }
 
 // batched prefill of `ids` (int32 device tensor) at start_position ..; writes K/V and hidden
-void prefill(torch::Tensor ids, torch::Tensor embed_weight, torch::Tensor layer_weights_packed,
-             torch::Tensor cos_table, torch::Tensor sin_table, torch::Tensor k_cache, torch::Tensor v_cache,
-             torch::Tensor hidden, int num_layers, int start_position, int max_seq_len, float attn_scale) {
+void check_prefill(const torch::Tensor& ids, const torch::Tensor& embed_weight, const torch::Tensor& layer_weights_packed,
+                   const torch::Tensor& cos_table, const torch::Tensor& sin_table, const torch::Tensor& k_cache,
+                   const torch::Tensor& v_cache, const torch::Tensor& hidden, int num_layers, int start_position,
+                   int max_seq_len) {
   check_dev(ids, "ids", torch::kInt32);
   const int64_t n = ids.numel();
   TORCH_CHECK(n >= 1, "prefill needs at least one id");
@@ -249,11 +251,35 @@ void prefill(torch::Tensor ids, torch::Tensor embed_weight, torch::Tensor layer_
   check_dev(k_cache, "k_cache", torch::kHalf, (int64_t)num_layers * NKV * max_seq_len * HD);
   check_dev(v_cache, "v_cache", torch::kHalf, (int64_t)num_layers * NKV * max_seq_len * HD);
   check_dev(hidden, "hidden", torch::kHalf, H);
-  check_rc(qwen_prefill(ids.data_ptr<int>(), (int)n, embed_weight.data_ptr(),
+}
+
+void prefill(torch::Tensor ids, torch::Tensor embed_weight, torch::Tensor layer_weights_packed,
+             torch::Tensor cos_table, torch::Tensor sin_table, torch::Tensor k_cache, torch::Tensor v_cache,
+             torch::Tensor hidden, int num_layers, int start_position, int max_seq_len, float attn_scale) {
+  check_prefill(ids, embed_weight, layer_weights_packed, cos_table, sin_table, k_cache, v_cache, hidden, num_layers,
+                start_position, max_seq_len);
+  check_rc(qwen_prefill(ids.data_ptr<int>(), (int)ids.numel(), embed_weight.data_ptr(),
                         reinterpret_cast<const LDGLayerWeight*>(layer_weights_packed.data_ptr()),
                         cos_table.data_ptr(), sin_table.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                         hidden.data_ptr(), num_layers, start_position, max_seq_len, attn_scale, stream_of(ids)),
            "prefill");
+}
+
+torch::Tensor prefill_hidden(torch::Tensor ids, torch::Tensor embed_weight, torch::Tensor layer_weights_packed,
+                             torch::Tensor final_norm_weight, torch::Tensor cos_table, torch::Tensor sin_table,
+                             torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor hidden, int num_layers,
+                             int start_position, int max_seq_len, float attn_scale) {
+  check_prefill(ids, embed_weight, layer_weights_packed, cos_table, sin_table, k_cache, v_cache, hidden, num_layers,
+                start_position, max_seq_len);
+  check_dev(final_norm_weight, "final_norm_weight", torch::kHalf, H);
+  auto rows = torch::empty({ids.numel(), H}, hidden.options());
+  check_rc(qwen_prefill_hidden(ids.data_ptr<int>(), (int)ids.numel(), embed_weight.data_ptr(),
+                               reinterpret_cast<const LDGLayerWeight*>(layer_weights_packed.data_ptr()),
+                               final_norm_weight.data_ptr(), cos_table.data_ptr(), sin_table.data_ptr(), k_cache.data_ptr(),
+                               v_cache.data_ptr(), hidden.data_ptr(), rows.data_ptr(), num_layers, start_position,
+                               max_seq_len, attn_scale, stream_of(ids)),
+           "prefill_hidden");
+  return rows;
 }
 
 // wall-clock ticks at the start and every grid barrier of the last prefill (profiling aid)
@@ -372,8 +398,11 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> cross_entropy(const torc
   const auto f32 = torch::dtype(torch::kFloat).device(hidden.device());
   auto loss = torch::empty({a.tokens}, f32), lse = torch::empty({a.tokens}, f32);
   torch::Tensor total;
-  if (want_total) total = a.tokens ? torch::empty({2}, f32) : torch::zeros({2}, f32);
-  if (a.tokens == 0) return {loss, lse, total};
+  if (want_total) total = torch::empty({3}, f32);
+  if (a.tokens == 0) {
+    if (want_total) total.copy_(torch::tensor({0.f, 0.f, NAN}));  // (a mean of nothing)
+    return {loss, lse, total};
+  }
   const auto ws = workspace_of(qwen_cross_entropy_workspace(a.tokens, a.vocab, a.width), hidden);
   check_rc(qwen_cross_entropy(hidden.data_ptr(), a.hidden_ld, weight.data_ptr(), a.weight_ld, a.targets.data_ptr(),
                               a.target_bits, a.tokens, a.vocab, a.width, a.dtype, ignore_index, loss.data_ptr<float>(),
@@ -396,7 +425,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> lm_head_cross_entropy_to
 
 std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> lm_head_cross_entropy_backward(
     torch::Tensor grad_loss, torch::Tensor hidden, torch::Tensor weight, torch::Tensor targets, torch::Tensor loss,
-    torch::Tensor lse, int64_t ignore_index, bool need_hidden, bool need_weight) {
+    torch::Tensor lse, int64_t ignore_index, bool need_hidden, bool need_weight, c10::optional<torch::Tensor> divisor) {
   const c10::DeviceGuard guard(hidden.device());
   const HeadArgs a = check_head(hidden, weight, targets);
   TORCH_CHECK(grad_loss.is_cuda() && grad_loss.scalar_type() == torch::kFloat && grad_loss.dim() == 1 &&
@@ -406,13 +435,18 @@ std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> lm_head_c
     TORCH_CHECK(t.device() == hidden.device() && t.scalar_type() == torch::kFloat && t.dim() == 1 && t.size(0) == a.tokens &&
                     t.is_contiguous(),
                 "loss and lse must be the contiguous float32 GPU tensors of ", a.tokens, " entries that the forward call gave");
+  if (divisor.has_value()) {
+    TORCH_CHECK(divisor->device() == hidden.device() && divisor->scalar_type() == torch::kFloat && divisor->numel() == 1,
+                "divisor must be one float32 number on hidden's device");
+  }
   c10::optional<torch::Tensor> gh, gw;
   if (need_hidden) gh = torch::empty({a.tokens, a.width}, hidden.options());
   if (need_weight) gw = a.tokens ? torch::empty({a.vocab, a.width}, weight.options()) : torch::zeros({a.vocab, a.width}, weight.options());
   if (a.tokens == 0 || (!need_hidden && !need_weight)) return {gh, gw};
   const auto ws = workspace_of(qwen_cross_entropy_backward_workspace(a.tokens, a.vocab, a.width, need_hidden, need_weight), hidden);
-  check_rc(qwen_cross_entropy_backward(grad_loss.data_ptr<float>(), a.tokens == 1 ? 0 : grad_loss.stride(0), hidden.data_ptr(),
-                                       a.hidden_ld, weight.data_ptr(), a.weight_ld, a.targets.data_ptr(), a.target_bits,
+  check_rc(qwen_cross_entropy_backward(grad_loss.data_ptr<float>(), a.tokens == 1 ? 0 : grad_loss.stride(0),
+                                       divisor.has_value() ? divisor->data_ptr<float>() : nullptr, hidden.data_ptr(), a.hidden_ld,
+                                       weight.data_ptr(), a.weight_ld, a.targets.data_ptr(), a.target_bits,
                                        a.tokens, a.vocab, a.width, a.dtype, ignore_index, loss.data_ptr<float>(),
                                        lse.data_ptr<float>(), need_hidden ? gh->data_ptr() : nullptr, need_weight ? gw->data_ptr() : nullptr,
                                        ws.data_ptr(), ws.numel(), stream_of(hidden)),
@@ -504,12 +538,13 @@ PYBIND11_MODULE(qwen_megakernel_C, m) {
         "cross entropy of hidden rows against the head's rows, without keeping the logits -> (loss, lse)",
         pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("ignore_index") = -100);
   m.def("lm_head_cross_entropy_total", &lm_head_cross_entropy_total,
-        "lm_head_cross_entropy, and [sum of the losses, positions that count]", pybind11::arg("hidden"),
+        "lm_head_cross_entropy, and [sum of the losses, positions that count, mean]", pybind11::arg("hidden"),
         pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("ignore_index") = -100);
   m.def("lm_head_cross_entropy_backward", &lm_head_cross_entropy_backward,
         "its gradients -> (grad_hidden, grad_weight), None for one that is not needed", pybind11::arg("grad_loss"),
         pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("loss"), pybind11::arg("lse"),
-        pybind11::arg("ignore_index") = -100, pybind11::arg("need_hidden") = true, pybind11::arg("need_weight") = true);
+        pybind11::arg("ignore_index") = -100, pybind11::arg("need_hidden") = true, pybind11::arg("need_weight") = true,
+        pybind11::arg("divisor") = pybind11::none());
   m.def("quantize_rows", &quantize_rows, "rows to 8-bit integers with a scale each -> (q, scale)", pybind11::arg("x"));
   m.def("matmul_i8", &matmul_i8, "product of 8-bit rows: out[t, n] = a_scale[t] b_scale[n] sum_k a[t, k] b[n, k]",
         pybind11::arg("a"), pybind11::arg("a_scale"), pybind11::arg("b"), pybind11::arg("b_scale"),
@@ -522,6 +557,11 @@ PYBIND11_MODULE(qwen_megakernel_C, m) {
         pybind11::arg("cos_table"), pybind11::arg("sin_table"), pybind11::arg("k_cache"), pybind11::arg("v_cache"),
         pybind11::arg("hidden"), pybind11::arg("num_layers"), pybind11::arg("start_position"),
         pybind11::arg("max_seq_len"), pybind11::arg("attn_scale"));
+  m.def("prefill_hidden", &prefill_hidden, "prefill that returns the final-normed hidden row of every position",
+        pybind11::arg("ids"), pybind11::arg("embed_weight"), pybind11::arg("layer_weights_packed"),
+        pybind11::arg("final_norm_weight"), pybind11::arg("cos_table"), pybind11::arg("sin_table"),
+        pybind11::arg("k_cache"), pybind11::arg("v_cache"), pybind11::arg("hidden"), pybind11::arg("num_layers"),
+        pybind11::arg("start_position"), pybind11::arg("max_seq_len"), pybind11::arg("attn_scale"));
   m.def("sample", &sample, "one token from fp32 logits: temperature, top-k, top-p, Philox Gumbel-max draw",
         pybind11::arg("logits"), pybind11::arg("temperature"), pybind11::arg("top_k") = 0,
         pybind11::arg("top_p") = 1.0, pybind11::arg("seed") = 0, pybind11::arg("step") = 0);
