@@ -564,14 +564,18 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) matmul_i8_kernel(Prod
   run_product<C>(P, ring, epi);
 }
 
-// Rows to 8-bit integers: scale = max |x| / 127, q = 127 x / max |x| rounded to the nearest integer, ties to even.
-// x has at most 11 significant bits, so 127 x is exact in fp32, and where 127 x / max |x| is not
-// k + 1/2 itself it differs from it by more than 2^-18 of its size: the fp32 division rounds to the same
-// integer as the exact quotient. A row of zeros gets scale 0; one with an infinity or a NaN scale NaN and
-// zeros, so that what is computed from it is NaN. One wave per row.
-template <class T>
+// Rows to 8-bit integers: scale = max |x| / 127, q = 127 x / max |x| rounded to the nearest integer, ties to even:
+// exactly, without a division per number. x and max |x| have at most 11 significant bits, so a quotient that is
+// not k + 1/2 itself differs from it by more than 2^-19 of its size (|254 x - (2 k + 1) max| is a whole number of
+// steps of x or max, and 254 * 2047 < 2^19). t = x * fl(127 / max) is good to 2^-23; rounded to 20 bits it is k + 1/2 where
+// the quotient is, and on the quotient's side of it where it is not. A row of zeros gets scale 0; one with an
+// infinity or a NaN scale NaN and zeros, so that what is computed from it is NaN. One wave per row, the row
+// in registers up to 2048 numbers. Bound by memory: 151936 rows of 1024 in 80 us, 5.8 TB/s (127 us with a
+// division per number and the row read twice).
+template <class T, int CHUNKS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long ld, int rows, int width, signed char* q,
                                                             float* scale) {
+#pragma clang fp contract(off)
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= rows) return;
   typedef T t8 __attribute__((ext_vector_type(8)));
@@ -579,31 +583,58 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long ld,
   signed char* out = q + (long)row * width;
   float top = 0.f;
   bool bad = false;
-  for (int c = 8 * lane; c < width; c += 512) {
-    const t8 v = *(const t8*)(p + c);
+  auto look = [&](const t8& v) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float a = fabsf((float)v[k]);
       bad |= !(a < INFINITY);
       top = fmaxf(top, a);
     }
+  };
+  t8 held[CHUNKS > 0 ? CHUNKS : 1];
+  if (CHUNKS > 0) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) held[c] = *(const t8*)(p + min(8 * lane + 512 * c, width - 8));
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) look(held[c]);
+  } else {
+    for (int c = 8 * lane; c < width; c += 512) look(*(const t8*)(p + c));
   }
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   bad = __any(bad);
   if (lane == 0) scale[row] = bad ? NAN : top / 127.f;
-  // (bf16: 127 x could pass fp32's range; a power of two leaves every quotient as it is)
-  const float f = top > 0x1p100f ? 0x1p-20f : 1.f, d = bad || top == 0.f ? INFINITY : top * f;
-  for (int c = 8 * lane; c < width; c += 512) {
-    const t8 v = *(const t8*)(p + c);
-    unsigned long long w = 0;
+  // powers of two keep 127 / max and x in fp32's range at both ends of bf16's, and leave every quotient as it is
+  const float f = top > 0x1p60f ? 0x1p-60f : top < 0x1p-60f ? 0x1p66f : 1.f;
+  const float r = top == 0.f || bad ? 0.f : 127.f / (top * f);
+  auto round = [&](const t8& v, int at) {
+    u32 w[2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float y = bad ? 0.f : rintf((float)v[k] * f * 127.f / d);
-      w |= (unsigned long long)(unsigned char)(signed char)(int)y << (8 * k);
+    for (int h = 0; h < 2; ++h) {
+      u32 b[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float t = (float)v[4 * h + k] * f * r, c = 17.f * t, t20 = c - (c - t);
+        b[k] = __float_as_uint(t20 + 12582912.f);  // (1.5 * 2^23: the sum's low byte is the integer)
+      }
+      w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u),
+                                   0x05040100u);
+      if (bad) w[h] = 0;
     }
-    *(unsigned long long*)(out + c) = w;
+    *(unsigned long long*)(out + at) = (unsigned long long)w[1] << 32 | w[0];
+  };
+  if (CHUNKS > 0) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+      if (8 * lane + 512 * c < width) round(held[c], 8 * lane + 512 * c);
+  } else {
+    for (int c = 8 * lane; c < width; c += 512) round(*(const t8*)(p + c), c);
   }
+}
+template <class T>
+const void* quantize_kernel(int width) {
+  return width <= 1024 ? (const void*)quantize_rows_kernel<T, 2>
+         : width <= 2048 ? (const void*)quantize_rows_kernel<T, 4> : (const void*)quantize_rows_kernel<T, 0>;
 }
 
 // ---- the engine's final norm over many rows --------------------------------------------
@@ -986,8 +1017,8 @@ extern "C" int qwen_quantize_rows(const void* x, long long stride, int rows, int
   if (!x || !q || !scale || !aligned16(x) || !aligned16(q)) return QWEN_ERR_ARG;
   long ld = (long)stride;
   void* args[] = {&x, &ld, &rows, &width, &q, &scale};
-  return launch(dtype == QWEN_F16 ? (const void*)quantize_rows_kernel<_Float16> : (const void*)quantize_rows_kernel<__bf16>,
-                ((long)rows + 3) / 4, 256, args, stream);
+  return launch(dtype == QWEN_F16 ? quantize_kernel<_Float16>(width) : quantize_kernel<__bf16>(width), ((long)rows + 3) / 4, 256,
+                args, stream);
 }
 
 namespace hd {
