@@ -3,7 +3,9 @@
 // None of their kernels waits for another workgroup; they may run beside anything.
 #include <hip/hip_runtime.h>
 #include <cstdint>
+#include <tuple>
 #include <type_traits>
+#include <utility>
 
 #include "qwen_megakernel.h"
 
@@ -443,6 +445,7 @@ __global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part
   if (tile >= tiles_t * tiles_n || t >= tokens || n >= width) return;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
   if (targets[t] != targets.ignore) {
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) a += *(const f32x4*)(part + ((long)s * tiles_t * tiles_n * PER_TILE + e) * 4);
     a *= grad[t] * unscale;
   }
@@ -710,15 +713,19 @@ struct StatsTiles {  // (no stores through LDS: a deeper ring)
 // the chip, each as long as its numbers at the rate that this tile reaches (measured on 1919 positions: 16-bit 1622, 921
 // and 562 us, 8-bit 909, 510 and 343).
 template <class C>
-long cost(int tokens, int rows, int splits, int percent) {
-  const long items = (long)splits * ((tokens + C::BT - 1) / C::BT) * ((rows + C::BN - 1) / C::BN);
+long cost(int tokens, int rows, int percent) {
+  const long items = (long)((tokens + C::BT - 1) / C::BT) * ((rows + C::BN - 1) / C::BN);
   const long rounds = (items + CUS * C::OCC - 1) / (CUS * C::OCC);
   return rounds * C::OCC * C::BN * C::BT * 100 / percent;
 }
 template <class TS>
+long tile_cost(TileKind k, int tokens, int rows) {
+  return k == SMALL ? cost<typename TS::Small>(tokens, rows, 36) : k == MIDDLE ? cost<typename TS::Middle>(tokens, rows, 62)
+                                                                                : cost<typename TS::Large>(tokens, rows, 100);
+}
+template <class TS>
 TileKind pick(int tokens, int rows) {
-  const long s = cost<typename TS::Small>(tokens, rows, 1, 36), m = cost<typename TS::Middle>(tokens, rows, 1, 62),
-             l = cost<typename TS::Large>(tokens, rows, 1, 100);
+  const long s = tile_cost<TS>(SMALL, tokens, rows), m = tile_cost<TS>(MIDDLE, tokens, rows), l = tile_cost<TS>(LARGE, tokens, rows);
   return l <= m && l <= s ? LARGE : m <= s ? MIDDLE : SMALL;
 }
 // f(tile) for the tile of this kind
@@ -833,18 +840,46 @@ struct BackwardPlan {
   int tokens_pad;   // K of grad_weight's product
   int rows;         // vocabulary rows per piece (a multiple of 256)
   TileKind kind;    // of grad_hidden's product (its partial sums are laid out by tile)
-  int splits, split_steps;
+  int splits;
   long g, weighted, partial, top, bytes;  // places in the workspace
 };
+// K steps in at most `most` parts: their length, their number
+std::pair<int, int> split(int steps, int most) {
+  const int length = (steps + most - 1) / most;
+  return {length, (steps + length - 1) / length};
+}
+
+// the cost of one piece's products, and of what comes with a piece (launches, partial sums read and written)
+long piece_cost(const Head& h, int rows, bool want_weight) {
+  typedef Tiles<Half> G;
+  typedef Tiles<Half, COLS, COLS> W;
+  const long k = 1024 / 16;  // in units of 16 numbers of k
+  return tile_cost<G>(pick<G>(h.tokens, rows), h.tokens, rows) * (h.width / 8) / 2 +
+         (want_weight ? tile_cost<W>(pick<W>(rows, h.width), rows, h.width) * (h.tokens + 15) / 16 : 0) + 256 * 256 * k / 3;
+}
 BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
   typedef Tiles<Half, COLS, ROWS> TS;
   BackwardPlan b;
   b.tokens_pad = (int)round_up(h.tokens, 64);
-  // the gradient of the logits is kept for a piece of the vocabulary: 128 MB, half of the 256 MB cache before HBM
-  // (4096 positions: 64 MB 4380 us, 128 MB 3845, 256 MB 3977)
+  // The gradient of the logits is kept for a piece of the vocabulary: at most 128 MB, half of the 256 MB cache before HBM
+  // (4096 positions: 64 MB 4380 us, 128 MB 3845, 256 MB 3977). Within that, the size whose products leave the
+  // fewest CUs idle in their last rounds (999 positions 1104 -> 986 us). Pieces of which the head's rows fit the
+  // cache too, for the second product that reads them, are no faster (20 positions 224 us instead of 207).
   constexpr long PIECE = 64L << 20;
-  const long rows = PIECE / b.tokens_pad / 256 * 256, all = round_up(h.vocab, 256);
-  b.rows = (int)(rows < 256 ? 256 : rows > all ? all : rows);
+  const long all = round_up(h.vocab, 256);
+  long most = PIECE / b.tokens_pad / 256 * 256;
+  most = most < 256 ? 256 : most > all ? all : most;
+  b.rows = (int)most;
+  long least = -1;
+  for (long rows = most; rows >= 256 && rows > most / 2; rows -= 256 * (1 + most / 65536)) {
+    const long full = h.vocab / rows;
+    const int last = (int)(h.vocab - full * rows);
+    const long c = full * piece_cost(h, (int)rows, want_weight) + (last ? piece_cost(h, last, want_weight) : 0);
+    if (least < 0 || c < least) {
+      least = c;
+      b.rows = (int)rows;
+    }
+  }
   // of grad_hidden's sums over the vocabulary, as many parts as give every workgroup one
   const int steps = (int)(round_up(b.rows < h.vocab ? b.rows : h.vocab, 64) / 64);  // of the first piece; no other has more
   b.kind = h.tokens <= 64 ? SMALL : h.tokens <= 128 ? MIDDLE : LARGE;
@@ -854,8 +889,7 @@ BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
     b.splits = (int)(s < 1 ? 1 : s > steps ? steps : s);
     return tiles * C::BN * C::BT;
   });
-  b.split_steps = (steps + b.splits - 1) / b.splits;
-  b.splits = (steps + b.split_steps - 1) / b.split_steps;
+  b.splits = split(steps, b.splits).second;
   long at = 0;
   auto take = [&](long bytes) {
     const long p = at;
@@ -922,8 +956,7 @@ int backward(const Head& h, Upstream grad, const float* loss, const float* lse, 
         typedef decltype(c) C;
         Product P = make_product<C>(Operand{(const char*)g, 2L * b.rows, tokens, 2 * rows_pad},
                                     Operand{w, 2 * h.weight_ld, width, rows}, rows_pad / 64);
-        P.split_steps = b.split_steps;
-        P.splits = (P.steps + P.split_steps - 1) / P.split_steps;
+        std::tie(P.split_steps, P.splits) = split(P.steps, b.splits);
         Partials<C> e;
         e.out = partial;
         e.add = v0 > 0;
@@ -932,7 +965,7 @@ int backward(const Head& h, Upstream grad, const float* loss, const float* lse, 
       if (rc != QWEN_OK) return rc;
     }
     if (grad_weight) {
-      rc = with_tile<Tiles<E, COLS, COLS>>(tokens <= 128 ? MIDDLE : LARGE, [&](auto c) {
+      rc = with_tile<Tiles<E, COLS, COLS>>(pick<Tiles<E, COLS, COLS>>(rows, width), [&](auto c) {
         typedef decltype(c) C;
         Product P = make_product<C>(Operand{(const char*)g, 2L * b.rows, rows_pad, tokens_pad},
                                     Operand{(const char*)weighted, 2L * width, width, tokens_pad}, tokens_pad / 64);
