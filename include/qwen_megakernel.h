@@ -307,7 +307,7 @@ int qwen_quantize_rows(const void* x, long long stride, int rows, int width, int
 /* Matrix product in 8-bit integers: out[t][n] = a_scale[t] b_scale[n] sum_k a[t][k] b[n][k], with
  * a int8 [tokens][width], b int8 [channels][width], out [tokens][channels] in out_dtype (QWEN_F16,
  * QWEN_BF16 or QWEN_F32). The sum is exact; the scaling is fp32, rounded once to out_dtype. width: a multiple
- * of 16, at most 65536; channels: at most 4194304; a, b and out 16-byte aligned. */
+ * of 16, at most 65536; tokens: at most 1048576; channels: at most 4194304; a, b and out 16-byte aligned. */
 int qwen_matmul_i8(const signed char* a, const float* a_scale, const signed char* b, const float* b_scale, void* out,
                    int out_dtype, int tokens, int channels, int width, hipStream_t stream);
 

@@ -880,13 +880,15 @@ BackwardPlan backward_plan(const Head& h, bool want_hidden, bool want_weight) {
       b.rows = (int)rows;
     }
   }
-  // of grad_hidden's sums over the vocabulary, as many parts as give every workgroup one
+  // of grad_hidden's sums over the vocabulary, as many parts as give every workgroup one, of 8 K steps at least (each
+  // is written and read again)
   const int steps = (int)(round_up(b.rows < h.vocab ? b.rows : h.vocab, 64) / 64);  // of the first piece; no other has more
   b.kind = h.tokens <= 64 ? SMALL : h.tokens <= 128 ? MIDDLE : LARGE;
   const long tile_numbers = with_tile<TS>(b.kind, [&](auto c) {
     typedef decltype(c) C;
     const long tiles = (long)((h.tokens + C::BT - 1) / C::BT) * ((h.width + C::BN - 1) / C::BN), s = CUS * C::OCC / tiles;
-    b.splits = (int)(s < 1 ? 1 : s > steps ? steps : s);
+    b.splits = (int)(s > steps / 8 ? steps / 8 : s);
+    if (b.splits < 1) b.splits = 1;
     return tiles * C::BN * C::BT;
   });
   b.splits = split(steps, b.splits).second;
@@ -1094,7 +1096,7 @@ int norm_rows(const float* x, const void* gain, int rows, void* out, hipStream_t
 extern "C" int qwen_matmul_i8(const signed char* a, const float* a_scale, const signed char* b, const float* b_scale,
                               void* out, int out_dtype, int tokens, int channels, int width, hipStream_t stream) {
   // 65536 products of 8-bit numbers stay within 2^30
-  if (tokens < 0 || channels < 0 || channels > MAX_CHANNELS || width < 16 || width % 16 != 0 || width > 65536) return QWEN_ERR_ARG;
+  if (tokens < 0 || tokens > MAX_TOKENS || channels < 0 || channels > MAX_CHANNELS || width < 16 || width % 16 != 0 || width > 65536) return QWEN_ERR_ARG;
   if (out_dtype != QWEN_F16 && out_dtype != QWEN_BF16 && out_dtype != QWEN_F32) return QWEN_ERR_ARG;
   if (tokens == 0 || channels == 0) return QWEN_OK;
   if (!a || !a_scale || !b || !b_scale || !out || !aligned16(a) || !aligned16(b) || !aligned16(out)) return QWEN_ERR_ARG;

@@ -462,6 +462,37 @@ def test_a_step_of_all_of_them_captured_and_replayed(ext):
         assert all(torch.equal(a, b) for a, b in zip(eager, captured2)), k
 
 
+def test_loss_and_gradients_captured_through_autograd(ext):
+    """A training step in a graph, its gradients taken with torch.autograd.grad; inputs change between replays."""
+    import Qwen06B_architecture as qa
+
+    h, w, y = make(200, 2003, 192, torch.float16, seed=17)
+    y[::4] = IGNORE
+
+    def step():
+        hx, wx = h.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = qa.lm_head_loss(hx, wx, y)
+        return (loss.detach(), *torch.autograd.grad(loss * 512.0, [hx, wx]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm up on the side, as torch asks for
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(3):
+        new = make(200, 2003, 192, torch.float16, seed=50 + k)
+        h.copy_(new[0])
+        w.copy_(new[1])
+        y[1::4] = new[2][1::4]
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, eager)), k
+
+
 def test_two_threads(ext):
     """Calls from two threads, each on a stream of its own."""
     import threading
@@ -598,6 +629,58 @@ def test_hidden_states_and_8_bit_logits(ext, decoder):
     w = decoder._lm_head_weight.double()
     bound = 0.5 * s[:, None] * w.abs().sum(dim=1) + 0.5 * head8[1].double() * (q.abs() * s[:, None]).sum(dim=1)[:, None]
     assert bool(((got.double() - exact).abs() <= 1.001 * bound + 1e-6).all())
+
+
+def test_hidden_states_captured_and_replayed(ext, decoder):
+    """The prefill and the norm that reads its workspace, as nodes of a graph between calls of other lengths."""
+    import qwen_weights as qw
+
+    d = decoder
+
+    def call(t, n):
+        return ext.prefill_hidden(t, d._embed_weight, d._layer_weights_packed, d._final_norm_weight, d._cos_table, d._sin_table,
+                                  d._k_cache, d._v_cache, d._hidden, d._num_layers, 0, 2048, d._attn_scale)
+
+    texts = [torch.tensor(qw.synthetic_prompt(150, seed=60 + k), dtype=torch.int32, device="cuda") for k in range(3)]
+    want = [call(t, 150).clone() for t in texts]
+    ids = texts[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        rows = call(ids, 150)
+    for k in (1, 2, 0, 1):
+        ids.copy_(texts[k])
+        graph.replay()
+        other = call(texts[(k + 1) % 3], 150)  # right after it, on the same workspace
+        torch.cuda.synchronize()
+        assert torch.equal(rows, want[k]) and torch.equal(other, want[(k + 1) % 3]), k
+    assert ext.last_error() == 0
+
+
+def test_two_streams_of_hidden_states(ext, decoder):
+    """The second call's prefill waits for the first one's norm, which reads the shared workspace."""
+    import qwen_weights as qw
+
+    ids = [qw.synthetic_prompt(n, seed=n) for n in (900, 880)]
+    caches = [(torch.zeros_like(decoder._k_cache), torch.zeros_like(decoder._v_cache)) for _ in ids]
+    hidden = [torch.empty_like(decoder._hidden) for _ in ids]
+    d = decoder
+
+    def call(k):
+        t = torch.tensor(ids[k], dtype=torch.int32, device="cuda")
+        return ext.prefill_hidden(t, d._embed_weight, d._layer_weights_packed, d._final_norm_weight, d._cos_table, d._sin_table,
+                                  *caches[k], hidden[k], d._num_layers, 0, 2048, d._attn_scale)
+
+    want = [call(0), call(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        got = []
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(call(k))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_decoder_refusals(decoder):

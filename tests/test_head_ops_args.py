@@ -92,6 +92,7 @@ def test_quantize_rows(lib, args):
     (A, A, A + 4, A, A, F16, 4, 4, 64), (A, A, A, A, A + 4, F16, 4, 4, 64), (A, A, A, A, A, 3, 4, 4, 64),
     (A, A, A, A, A, F16, -1, 4, 64), (A, A, A, A, A, F16, 4, -1, 64), (A, A, A, A, A, F16, 4, 4, 24),
     (A, A, A, A, A, F16, 4, 4, 0), (A, A, A, A, A, F16, 4, 4, 65552), (A, A, A, A, A, F16, 4, (1 << 22) + 1, 64),
+    (A, A, A, A, A, F16, (1 << 20) + 1, 4, 64),
 ])
 def test_matmul_i8(lib, args):
     assert lib.qwen_matmul_i8(*args, None) == ERR_ARG
