@@ -225,37 +225,13 @@ def _pack_layer_weights(layer_weights: list) -> torch.Tensor:
     return t_aligned
 
 
-class _HeadLoss(torch.autograd.Function):
-    """Cross entropy against the head: of every position, or their sum, or their mean."""
-
-    @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
-        loss, lse, total = qwen_megakernel_C.lm_head_cross_entropy_total(hidden, weight, targets, ignore_index)
-        # (total.data: a caller's in-place change of the scalar is not one of the count)
-        ctx.save_for_backward(hidden, weight, targets, loss, lse, total.data)
-        ctx.ignore_index = ignore_index
-        ctx.reduction = reduction
-        return loss if reduction == "none" else total[0 if reduction == "sum" else 2]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        hidden, weight, targets, loss, lse, total = ctx.saved_tensors
-        grads = qwen_megakernel_C.lm_head_cross_entropy_backward(
-            grad if ctx.reduction == "none" else grad.expand(loss.shape), hidden, weight, targets, loss, lse,
-            ctx.ignore_index, *ctx.needs_input_grad[:2], total[1] if ctx.reduction == "mean" else None)
-        return (*grads, None, None, None)
-
-
 def lm_head_loss(hidden, weight, targets, ignore_index: int = -100, reduction: str = "mean"):
     """Softmax cross entropy of hidden rows [n, width] against a head's rows [vocabulary, width] without keeping the
     logits, with gradients for both (fp16 or bf16; the loss is fp32). ``targets``: [n] int64 or int32, those equal
     to ``ignore_index`` do not count. ``reduction``: "mean" over the positions that count (NaN if none does, as
     0 / 0), "sum" or "none". fp16 gradients of a mean over many positions are small numbers: scale the loss, as
-    in any fp16 training."""
-    if reduction not in ("mean", "sum", "none"):
-        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
-    return _HeadLoss.apply(hidden, weight, targets, ignore_index, reduction)
+    in any fp16 training. First derivatives only."""
+    return _require_megakernel_op("lm_head_loss")(hidden, weight, targets, ignore_index, reduction)
 
 
 class Decoder:

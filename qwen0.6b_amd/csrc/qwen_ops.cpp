@@ -9,6 +9,7 @@
 // violation raises RuntimeError; the pointer-table alignment check of
 // qwen_ops.cpp:64-65 is kept.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -454,6 +455,49 @@ std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> lm_head_c
   return {gh, gw};
 }
 
+// lm_head_cross_entropy with autograd: every position's loss, or their sum, or their mean
+enum Reduction : int64_t { NONE, SUM, MEAN };
+struct HeadLoss : torch::autograd::Function<HeadLoss> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& hidden, const torch::Tensor& weight,
+                               const torch::Tensor& targets, int64_t ignore_index, int64_t reduction) {
+    torch::Tensor loss, lse, total;
+    std::tie(loss, lse, total) = cross_entropy(hidden, weight, targets, ignore_index, true);
+    ctx->save_for_backward({hidden, weight, targets, loss, lse, total});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["reduction"] = reduction;
+    if (reduction == NONE) return loss;
+    // a tensor of its own on the total's memory, not a view: callers may change their loss in place
+    return torch::empty({0}, total.options()).set_(total.storage(), reduction == SUM ? 0 : 2, {}, {});
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
+    c10::optional<torch::Tensor> divisor, gh, gw;
+    if (reduction == MEAN) divisor = v[5].select(0, 1);
+    {
+      const torch::NoGradGuard guard;
+      std::tie(gh, gw) = lm_head_cross_entropy_backward(reduction == NONE ? grads[0] : grads[0].expand({v[3].size(0)}), v[0], v[1],
+                                                        v[2], v[3], v[4], ctx->saved_data["ignore_index"].toInt(),
+                                                        ctx->needs_input_grad(0), ctx->needs_input_grad(1), divisor);
+    }
+    torch::autograd::variable_list out = {gh.value_or(torch::Tensor()), gw.value_or(torch::Tensor())};
+    if (torch::GradMode::is_enabled()) {  // a graph of this step was asked for: it ends here, with an error when it is used
+      for (auto& t : out)
+        if (t.defined()) t.requires_grad_();
+      out = (*std::make_shared<torch::autograd::DelayedError>("lm_head_loss has no second derivative", (int64_t)out.size()))(
+          std::move(out));
+    }
+    out.resize(5);
+    return out;
+  }
+};
+torch::Tensor lm_head_loss(torch::Tensor hidden, torch::Tensor weight, torch::Tensor targets, int64_t ignore_index,
+                           const std::string& reduction) {
+  TORCH_CHECK_VALUE(reduction == "mean" || reduction == "sum" || reduction == "none",
+                    "reduction must be 'mean', 'sum' or 'none', not '", reduction, "'");
+  return HeadLoss::apply(hidden, weight, targets, ignore_index, (int64_t)(reduction == "mean" ? MEAN : reduction == "sum" ? SUM : NONE));
+}
+
 std::tuple<torch::Tensor, torch::Tensor> quantize_rows(torch::Tensor x) {
   const c10::DeviceGuard guard(x.device());
   const int dtype = dtype_code(x.scalar_type(), "x");
@@ -545,6 +589,9 @@ PYBIND11_MODULE(qwen_megakernel_C, m) {
         pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("loss"), pybind11::arg("lse"),
         pybind11::arg("ignore_index") = -100, pybind11::arg("need_hidden") = true, pybind11::arg("need_weight") = true,
         pybind11::arg("divisor") = pybind11::none());
+  m.def("lm_head_loss", &lm_head_loss, "lm_head_cross_entropy with autograd: its mean, its sum or every position's",
+        pybind11::arg("hidden"), pybind11::arg("weight"), pybind11::arg("targets"), pybind11::arg("ignore_index") = -100,
+        pybind11::arg("reduction") = "mean");
   m.def("quantize_rows", &quantize_rows, "rows to 8-bit integers with a scale each -> (q, scale)", pybind11::arg("x"));
   m.def("matmul_i8", &matmul_i8, "product of 8-bit rows: out[t, n] = a_scale[t] b_scale[n] sum_k a[t, k] b[n, k]",
         pybind11::arg("a"), pybind11::arg("a_scale"), pybind11::arg("b"), pybind11::arg("b_scale"),

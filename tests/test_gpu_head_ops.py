@@ -304,6 +304,40 @@ def test_lm_head_loss(ext, dtype, reduction):
     assert torch.equal(only_w[0], gw)
 
 
+def test_lm_head_loss_changed_in_place_and_its_second_derivative(ext):
+    import Qwen06B_architecture as qa
+
+    h, w, y = make(50, 300, 64, torch.float16, seed=18)
+    h.requires_grad_()
+    for reduction in ("mean", "sum"):
+        want = torch.autograd.grad(qa.lm_head_loss(h, w, y, reduction=reduction) / 4, [h])[0]
+        loss = qa.lm_head_loss(h, w, y, reduction=reduction)
+        value = float(loss.detach())
+        loss /= 4
+        assert float(loss.detach()) == value / 4
+        assert torch.equal(torch.autograd.grad(loss, [h])[0], want)
+    # every position's losses are what the gradients are made of: changed in place, they are missed
+    loss = qa.lm_head_loss(h, w, y, reduction="none")
+    loss *= 2
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(loss.sum(), [h])
+    g, = torch.autograd.grad(qa.lm_head_loss(h, w, y), [h], create_graph=True)
+    with pytest.raises(RuntimeError):  # (torch's own: h is not in what is left of the graph)
+        torch.autograd.grad(g.float().sum(), [h], retain_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        (g.float().sum() + h.float().sum()).backward()
+    # nothing to differentiate, and no graph wanted
+    assert not qa.lm_head_loss(h.detach(), w, y).requires_grad
+    with torch.no_grad():
+        assert not qa.lm_head_loss(h, w, y).requires_grad
+    # accumulated over two calls, as a training loop does
+    h.grad = None
+    for _ in range(2):
+        (qa.lm_head_loss(h, w, y) * 64).backward()
+    one = torch.autograd.grad(qa.lm_head_loss(h, w, y) * 64, [h])[0]
+    assert torch.equal(h.grad, one + one)
+
+
 def dt_of(t):
     return t.dtype
 
