@@ -337,8 +337,18 @@ struct Stores {
 // * SCALE, in the inputs' 16-bit type: the next products take it as a matrix operand. fp16's SCALE (a power of
 // two, taken back at the end) keeps probabilities from 2^-29 on at full precision; without it those of a vocabulary
 // of 151936 would be subnormal. Tokens that do not count, and v past the vocabulary, get zeros.
+// The target's own entry is the largest of its token by far: its rounding is what one sees of G's. own_entry is that entry,
+// own_rest what its rounding leaves, which the gradients take up again (grad_hidden always, grad_weight for few tokens).
 template <class E>
 constexpr float grad_scale() { return sizeof(typename E::elem) == 2 && std::is_same<E, Half>::value ? 32768.f : 1.f; }
+
+template <class E>
+__device__ __forceinline__ float own_entry(float loss) { return expm1f(-loss) * grad_scale<E>(); }  // p - 1, also where p is nearly 1
+template <class E>
+__device__ __forceinline__ float own_rest(float loss) {
+  const float own = own_entry<E>(loss);
+  return own - (float)(typename E::elem)own;
+}
 
 // 4096 positions, bf16: 132 us for 16384 rows (1040 TFLOP/s); the stores, all workgroups' at once, are 16 of them.
 template <class C>
@@ -370,7 +380,7 @@ struct Softgrad : FromZero<C> {
         const float x = c ? loss[t] : 0.f;
         // (a NaN loss: a target that is no row of the head, or logits that are NaN)
         l2[j] = c ? (x == x ? fmaf(lse[t], LOG2E, -__builtin_log2f(SCALE)) : NAN) : 0.f;
-        own[j] = expm1f(-x) * SCALE;  // the target's p - 1, also where p is nearly 1
+        own[j] = own_entry<typename C::E>(x);
       }
     }
     const int n0 = at.tn * C::BN + 32 * C::NI * wn;
@@ -442,11 +452,14 @@ __global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_partials_kernel(
   run_product<C>(P, ring, epi);
 }
 
-// grad_hidden: the splits' sums in order, times the position's upstream gradient; a thread has 4 numbers of one row
+// grad_hidden: the splits' sums in order and what the target's entry lost to rounding, times the position's upstream gradient;
+// a thread has 4 numbers of one row
 template <class C>
 __global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part, int splits, int tiles_t, int tiles_n,
                                                                int tokens, int width, Targets targets, Upstream grad,
-                                                               float unscale, typename C::E::elem* out) {
+                                                               float unscale, const float* loss, int vocab,
+                                                               const typename C::E::elem* weight, long weight_ld,
+                                                               typename C::E::elem* out) {
   typedef typename C::E::elem T;
   constexpr int PER_TILE = C::BN * C::BT / 4;
   const long e = (long)blockIdx.x * 256 + threadIdx.x;
@@ -455,13 +468,19 @@ __global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part
   const int t = tile / tiles_n * C::BT + 32 * (C::NJ * (wave / C::WN) + ij % C::NJ) + (lane & 31);
   const int n = tile % tiles_n * C::BN + 32 * (C::NI * (wave % C::WN) + ij / C::NJ) + 8 * q + 4 * (lane >> 5);
   if (tile >= tiles_t * tiles_n || t >= tokens || n >= width) return;
+  typedef T t4 __attribute__((ext_vector_type(4)));
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
-  if (targets[t] != targets.ignore) {
+  const long long y = targets[t];
+  if (y != targets.ignore) {
+    if (y >= 0 && y < vocab) {
+      const t4 w = *(const t4*)(weight + y * weight_ld + n);
+      const float rest = own_rest<typename C::E>(loss[t]);
+      a = f32x4{rest * (float)w[0], rest * (float)w[1], rest * (float)w[2], rest * (float)w[3]};
+    }
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) a += *(const f32x4*)(part + ((long)s * tiles_t * tiles_n * PER_TILE + e) * 4);
     a *= grad[t] * unscale;
   }
-  typedef T t4 __attribute__((ext_vector_type(4)));
   *(t4*)(out + (long)t * width + n) = t4{(T)a[0], (T)a[1], (T)a[2], (T)a[3]};
 }
 
@@ -504,15 +523,66 @@ __global__ void __launch_bounds__(256) head_weighted_rows_kernel(const T* hidden
 }
 
 // grad_weight's rows of a piece. 4096 positions, bf16: 104 us for 16384 rows (1320 TFLOP/s, the matrix cores 63% busy).
-template <class C>
+// Of up to FEW tokens the target's entries are added what their rounding left; the lanes hold whose targets are
+// where, a wave adds a token's hidden row to the accumulators of the target's row. (Of more tokens the roundings'
+// errors are a fifth on top of the output's own.)
+// It is a kernel of its own (RESTS): it takes 20 of the last 27 registers of the 256x256 tile, and more positions have no use for it.
+constexpr int FEW = 256;  // (four targets a lane)
+template <class C, bool RESTS>
 struct WeightGrad : FromZero<C> {
   typedef typename C::E::elem T;
   T* out;  // [rows][width]
   Upstream grad;
   const float* top;  // as in head_weighted_rows_kernel
   int rows, width;
+  const T* weighted;  // [tokens][width]
+  const float* loss;
+  Targets targets;
+  int tokens, v0;  // (the piece's first row)
   char* lds;
+  bool looked = false;
+  int row0, row1, row2, row3;  // of tokens lane, 64 + lane, ..: the target's row of the piece, or -1 (a field each: an array would be in memory)
+  __device__ __forceinline__ void add_rests(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, int lane, int wn, int wt) {
+    if (!looked) {
+      looked = true;
+      const auto look = [&](int t) {
+        const long long y = t < tokens ? targets[t] : targets.ignore, far = y - v0;
+        return y != targets.ignore && far >= 0 && far < rows ? (int)far : -1;
+      };
+      row0 = look(lane), row1 = look(64 + lane), row2 = look(128 + lane), row3 = look(192 + lane);
+    }
+    const int r0 = at.tt * C::BT + 32 * C::NJ * wt;  // the wave's first row
+    const int n0 = at.tn * C::BN + 32 * C::NI * wn + 4 * (lane >> 5);
+    typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+      const int mine = q == 0 ? row0 : q == 1 ? row1 : q == 2 ? row2 : row3;
+      unsigned long long hits = __ballot(mine >= r0 && mine < r0 + 32 * C::NJ);
+      while (hits) {
+        const int l = __builtin_ctzll(hits);
+        hits &= hits - 1;
+        const int t = 64 * q + l, r = __builtin_amdgcn_readlane(mine, l) - r0;
+        const float rest = own_rest<typename C::E>(loss[t]);
+        const T* h = weighted + (long)t * width;
+        if ((lane & 31) != (r & 31)) continue;
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j)
+          if (j == r >> 5) {
+#pragma unroll
+            for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int n = n0 + 32 * i + 8 * k;
+                const t4 x = *(const t4*)(h + (n < width ? n : 0));  // (columns past the width are not stored)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][4 * k + e] = fmaf(rest, (float)x[e], acc[i][j][4 * k + e]);
+              }
+          }
+      }
+    }
+  }
   __device__ __forceinline__ void tile(f32x16 (&acc)[C::NI][C::NJ], const Cursor& at, bool, int lane, int wn, int wt) {
+    if constexpr (RESTS) add_rests(acc, at, lane, wn, wt);
     const float f = (top ? *top : fabsf(grad[0])) * (1.f / grad_scale<typename C::E>());
     Stores<C, T, true>::store(
         acc, at, lane, wn, wt, lds, out, width, rows, width,
@@ -523,8 +593,8 @@ struct WeightGrad : FromZero<C> {
         Nothing(), Nothing());
   }
 };
-template <class C>
-__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_weight_grad_kernel(Product P, WeightGrad<C> epi) {
+template <class C, bool RESTS>
+__global__ void __launch_bounds__(C::THREADS, C::PER_SIMD) head_weight_grad_kernel(Product P, WeightGrad<C, RESTS> epi) {
   __shared__ __align__(16) char ring[C::RING];
   __shared__ __align__(16) char stage[C::STAGING];
   epi.lds = stage + (threadIdx.x >> 6) * 4096;
@@ -985,13 +1055,22 @@ int backward(const Head& h, Upstream grad, const float* loss, const float* lse, 
         typedef decltype(c) C;
         Product P = make_product<C>(Operand{(const char*)g, 2L * b.rows, rows_pad, tokens_pad},
                                     Operand{(const char*)weighted, 2L * width, width, tokens_pad}, tokens_pad / 64);
-        WeightGrad<C> e;
-        e.out = (T*)grad_weight + (long)v0 * width;
-        e.grad = grad;
-        e.top = top;
-        e.rows = rows;
-        e.width = width;
-        return launch_product(head_weight_grad_kernel<C>, grid_of<C>(P), C::THREADS, P, e, stream);
+        const auto run = [&](auto rests) {
+          constexpr bool RESTS = decltype(rests)::value;
+          WeightGrad<C, RESTS> e;
+          e.out = (T*)grad_weight + (long)v0 * width;
+          e.grad = grad;
+          e.top = top;
+          e.rows = rows;
+          e.width = width;
+          e.weighted = weighted;
+          e.loss = loss;
+          e.targets = targets;
+          e.tokens = tokens;
+          e.v0 = v0;
+          return launch_product(head_weight_grad_kernel<C, RESTS>, grid_of<C>(P), C::THREADS, P, e, stream);
+        };
+        return tokens <= FEW ? run(std::true_type()) : run(std::false_type());
       });
       if (rc != QWEN_OK) return rc;
     }
@@ -1001,7 +1080,11 @@ int backward(const Head& h, Upstream grad, const float* loss, const float* lse, 
     typedef decltype(c) C;
     int splits = b.splits, tiles_t = (tokens + C::BT - 1) / C::BT, tiles_n = (width + C::BN - 1) / C::BN;
     float unscale = 1.f / grad_scale<E>();
-    void* a[] = {&partial, &splits, &tiles_t, &tiles_n, &tokens, &width, &targets, &grad, &unscale, &grad_hidden};
+    const void* weight = h.weight;
+    long weight_ld = h.weight_ld;
+    int vocab = h.vocab;
+    void* a[] = {&partial, &splits, &tiles_t, &tiles_n, &tokens, &width, &targets, &grad, &unscale, &loss, &vocab, &weight, &weight_ld,
+                 &grad_hidden};
     return launch((const void*)head_grad_hidden_kernel<C>, (long)tiles_t * tiles_n * (C::BN * C::BT / 1024), 256, a, stream);
   });
 }

@@ -272,6 +272,33 @@ def test_loss_of_a_target_that_is_nearly_certain(ext):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,vocab,width", [(1, 5003, 1024), (2, 1001, 512), (3, 151936, 1024), (7, 300, 264), (65, 4001, 512),
+                                                (256, 9001, 264), (700, 5003, 512)])
+def test_gradients_of_few_positions_have_one_rounding(ext, tokens, vocab, width, dtype):
+    """What G's rounding to 16 bits does to the targets' entries, the largest by far, is taken up again. With x the gradient
+    before its own rounding and e = x - want, the rounding takes x to the nearest number, so |got - x| <= |round(want) - x|
+    and |got - want| <= |round(want) - want| + 2 |e|. In norm, e is the other entries' roundings: each is off by at most
+    U of itself, in both directions alike and independently, so the squares add up, sum (U d w)^2 (a third of it on average).
+    The fp32 parts: logits up to 16, off by 2^-20 at most, move the entries by as much relative to them, and the sums add
+    some 2^-22; 2^-13 / 4, the least that one rounding leaves in norm, is 2^-15, so that 2 |e| grows by 0.08 of it at most."""
+    h, w, y = make(tokens, vocab, width, dtype, seed=70 + tokens, lean=4.0)
+    if tokens > 5:
+        y[4] = y[2]  # two positions with one target
+    fwd = ext.lm_head_cross_entropy(h, w, y)
+    scale = 1024.0  # (in fp16 small numbers would lose more than their rounding's half step)
+    gh, gw = ext.lm_head_cross_entropy_backward(torch.full((tokens,), scale, device="cuda"), h, w, y, *fwd)
+    d = torch.softmax(logits64(h, w), dim=1)
+    d[torch.arange(tokens), y] -= 1.0
+    other = d.clone()
+    other[torch.arange(tokens), y] = 0.0
+    for got, want, entries, rows in ((gh, scale * d @ w.double(), other, w),  # (past 256 positions grad_weight has them all)
+                                     (gw, scale * d.t().contiguous() @ h.double(), (other if tokens <= 256 else d).t().contiguous(), h)):
+        once = float((want.to(dtype).double() - want).norm())
+        e = U[dtype] * scale * float(((entries ** 2) @ (rows.double() ** 2)).sum().sqrt())
+        assert float((got.double() - want).norm()) <= 1.08 * once + 2 * e
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_lm_head_loss(ext, dtype, reduction):
     import Qwen06B_architecture as qa
