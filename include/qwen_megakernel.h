@@ -289,7 +289,8 @@ int qwen_cross_entropy(const void* hidden, long long hidden_stride, const void* 
  * Positions that do not count take no part (their hidden rows may hold anything) and get a zero row; those with a
  * NaN loss give NaN.
  * The logits are computed again, a piece of the vocabulary at a time; p - [v = target] is rounded to the inputs' dtype
- * for the matrix cores, sums are fp32, one rounding at the end. Same limits; tokens >= 1. */
+ * for the matrix cores (what the target's entry, the largest, loses is added again to grad_hidden, and to grad_weight of
+ * up to 256 positions), sums are fp32, one rounding at the end. Same limits; tokens >= 1. */
 long long qwen_cross_entropy_backward_workspace(int tokens, int vocab, int width, int want_hidden, int want_weight);
 int qwen_cross_entropy_backward(const float* grad_loss, long long grad_stride, const float* grad_divisor,
                                 const void* hidden, long long hidden_stride, const void* weight, long long weight_stride,

@@ -475,7 +475,8 @@ __global__ void __launch_bounds__(256) head_grad_hidden_kernel(const float* part
     if (y >= 0 && y < vocab) {
       const t4 w = *(const t4*)(weight + y * weight_ld + n);
       const float rest = own_rest<typename C::E>(loss[t]);
-      a = f32x4{rest * (float)w[0], rest * (float)w[1], rest * (float)w[2], rest * (float)w[3]};
+      // (none: nothing is added, also where the row holds the infinity that made the target impossible)
+      if (rest != 0.f) a = f32x4{rest * (float)w[0], rest * (float)w[1], rest * (float)w[2], rest * (float)w[3]};
     }
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) a += *(const f32x4*)(part + ((long)s * tiles_t * tiles_n * PER_TILE + e) * 4);

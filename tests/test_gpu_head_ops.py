@@ -299,6 +299,26 @@ def test_gradients_of_few_positions_have_one_rounding(ext, tokens, vocab, width,
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_an_impossible_target(ext, dtype):
+    """A target whose row holds the lowest infinity: its loss is infinite, its entry -1 exactly, the gradient by the formula."""
+    h, w, y = make(1, 300, 264, dtype, seed=5)
+    h[0, 40] = 2.0
+    w[y[0], 40] = -math.inf
+    loss, lse = ext.lm_head_cross_entropy(h, w, y)
+    gh, gw = ext.lm_head_cross_entropy_backward(torch.ones(1, device="cuda"), h, w, y, loss, lse)
+    d = torch.softmax(logits64(h, w), dim=1)
+    assert float(loss[0]) == math.inf and float(d[0, y[0]]) == 0.0
+    assert float(gh[0, 40]) == math.inf  # -1 times the row's -inf
+    d[0, y[0]] = -1.0
+    want = d @ w.double()
+    keep = torch.arange(264, device="cuda") != 40
+    # each other entry is off by its rounding and by the sums' (2 n + 8) 2^-24, the result by a rounding (fp16: or 2^-25)
+    tol = (U[dtype] + 2.0 ** -14) * (d.abs() @ w.double().abs()) + U[dtype] * want.abs() + 2.0 ** -25
+    assert bool(((gh.double() - want).abs() <= tol)[0, keep].all())
+    assert torch.equal(gw[y[0]], -h[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_lm_head_loss(ext, dtype, reduction):
     import Qwen06B_architecture as qa
