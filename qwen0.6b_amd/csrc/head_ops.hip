@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(256) head_weighted_rows_kernel(const T* hidden
 // Of up to FEW tokens the target's entries are added what their rounding left; the lanes hold whose targets are
 // where, a wave adds a token's hidden row to the accumulators of the target's row. (Of more tokens the roundings'
 // errors are a fifth on top of the output's own.)
-// It is a kernel of its own (RESTS): it takes 20 of the last 27 registers of the 256x256 tile, and more positions have no use for it.
+// It is a kernel of its own (RESTS): it takes 19 (fp16) or 26 (bf16) of the 27 registers that the 256x256 tile leaves.
 constexpr int FEW = 256;  // (four targets a lane)
 template <class C, bool RESTS>
 struct WeightGrad : FromZero<C> {
